@@ -87,6 +87,16 @@ typedef struct ScaPagedParams {
     int64_t layer;
 } ScaPagedParams;
 
+/* sca::PagedVarlenParams (paged_attention.hpp; no reference counterpart). */
+typedef struct ScaPagedVarlenParams {
+    const int64_t* seq_ids;      /* host; NULL => 0, 1, ... */
+    const int32_t* kv_lens;      /* host; NULL => the cache's lengths */
+    int64_t num_seqs;
+    int64_t layer;
+    const int32_t* page_table;   /* device; NULL => the cache's own */
+    int64_t max_blocks_per_seq;  /* of that table */
+} ScaPagedVarlenParams;
+
 typedef struct ScaTensor ScaTensor;           /* sci::Tensor */
 typedef struct ScaPagedKV ScaPagedKV;         /* sca::PagedKVCache */
 typedef struct ScaBlockManager ScaBlockManager; /* sca::BlockManager */
@@ -133,10 +143,15 @@ SCA_CAPI int sca_paged_decode_plan(const int64_t* lengths, int64_t batch, int64_
                                    int32_t* slot_waves);
 
 /* ---- KV helpers (kv_cache.hpp:97-110) ---- */
+/* sca::KvStorage of the *_stored functions: 0 in the cache's dtype, 1 e4m3 codes with exponent bytes
+ * (no reference counterpart). The plain ones stand for storage 0. */
 SCA_CAPI int sca_compute_slot_mapping(const int32_t* row, int64_t seq_start, int64_t num_tokens,
                                       int64_t block_size, int64_t max_blocks, int32_t* slots);
 SCA_CAPI int sca_kv_cache_bytes(const ScaKvConfig* cfg, uint64_t* bytes);
 SCA_CAPI int64_t sca_max_blocks_for_budget(const ScaKvConfig* cfg, uint64_t budget_bytes);
+SCA_CAPI int sca_kv_cache_bytes_stored(const ScaKvConfig* cfg, int32_t storage, uint64_t* bytes);
+SCA_CAPI int64_t sca_max_blocks_for_budget_stored(const ScaKvConfig* cfg, int32_t storage,
+                                                  uint64_t budget_bytes);
 
 /* ---- tensors (sci::Tensor) ---- */
 SCA_CAPI ScaTensor* sca_tensor_new(const int64_t* dims, int32_t ndims, int32_t dtype,
@@ -168,6 +183,7 @@ SCA_CAPI void sca_explain_tensors(const ScaTensor* q, const ScaTensor* k, const 
 
 /* ---- paged KV cache (paged_kv_cache.hpp:20-68, paged_attention.hpp:23-31) ---- */
 SCA_CAPI ScaPagedKV* sca_pkv_create(const ScaKvConfig* cfg, int32_t device_kind);
+SCA_CAPI ScaPagedKV* sca_pkv_create_stored(const ScaKvConfig* cfg, int32_t storage, int32_t device_kind);
 SCA_CAPI void sca_pkv_destroy(ScaPagedKV* c);
 SCA_CAPI int sca_pkv_append(ScaPagedKV* c, int64_t seq_id, int64_t layer, const ScaTensor* k_new,
                             const ScaTensor* v_new, void* stream);
@@ -202,6 +218,9 @@ SCA_CAPI uint64_t sca_pkv_synced_revision(const ScaPagedKV* c);
 SCA_CAPI void sca_pkv_stats(const ScaPagedKV* c, ScaKvStats* out);
 SCA_CAPI void* sca_pkv_layer_k(const ScaPagedKV* c, int64_t layer);
 SCA_CAPI void* sca_pkv_layer_v(const ScaPagedKV* c, int64_t layer);
+/* Exponent bytes of 8-bit storage (NULL otherwise). */
+SCA_CAPI void* sca_pkv_layer_k_exponents(const ScaPagedKV* c, int64_t layer);
+SCA_CAPI void* sca_pkv_layer_v_exponents(const ScaPagedKV* c, int64_t layer);
 /* The cache's BlockManager (borrowed; valid while the cache lives). */
 SCA_CAPI const ScaBlockManager* sca_pkv_blocks(const ScaPagedKV* c);
 /* KVCache::GatherK / GatherV of the cache's storage; ids are device int32. */
@@ -210,6 +229,11 @@ SCA_CAPI int sca_pkv_gather(const ScaPagedKV* c, int32_t is_key, int64_t layer,
                             ScaTensor** out);
 SCA_CAPI int sca_run_paged(const ScaTensor* q, const ScaPagedKV* kv, const ScaPagedParams* params,
                            const ScaConfig* cfg, ScaTensor** out, ScaStats* stats);
+/* sca::paged_attention_varlen: packed q [T, H_q, D], cfg->cu_seqlens_q on the host; *lse receives a new
+ * [T, H_q] tensor when cfg->return_lse. */
+SCA_CAPI int sca_run_paged_varlen(const ScaTensor* q, const ScaPagedKV* kv,
+                                  const ScaPagedVarlenParams* params, const ScaConfig* cfg,
+                                  ScaTensor** out, ScaTensor** lse, ScaStats* stats);
 
 /* ---- BlockManager (block_manager.hpp:31-61) ---- */
 SCA_CAPI ScaBlockManager* sca_bm_create(int64_t num_blocks, int64_t max_num_seqs,

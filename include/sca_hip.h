@@ -266,6 +266,67 @@ SCA_HIP_API int sca_hip_decode_splitk_paged(const sca_decode_params* params, voi
  * different streams) race; calls ordered on one stream are safe. */
 SCA_HIP_API int sca_hip_decode_splitk_noalloc(const sca_decode_params* params, void* stream);
 
+/* Decode over 8-bit pages (sca_kv8_layer below; no reference counterpart). `base` as for
+ * sca_hip_decode_splitk_paged, with k and v the code bytes of the layer (strides in bytes, multiples of
+ * 16), q and out fp16 or bf16, page_table set and block_size a power of two of at least 8; k_exp and
+ * v_exp are the layer's exponent bytes, whose pages hold num_kv_heads * block_size bytes. The partial
+ * scratch, the longest-first schedule and slot_waves (0 = 1) are those of the 16-bit decode. */
+typedef struct sca_decode8_params {
+    sca_decode_params base;
+    const uint8_t* k_exp;
+    const uint8_t* v_exp;
+} sca_decode8_params;
+
+SCA_HIP_API int sca_hip_decode8_paged(const sca_decode8_params* params, void* stream);
+
+/* ------------------------------------------------------------------------------------------- */
+/* attention of ragged chunks of new tokens over paged KV (no reference counterpart: the        */
+/* reference attends pages with one query token per sequence)                                   */
+/* ------------------------------------------------------------------------------------------- */
+/* Sequence s has new tokens [cu_seqlens_q[s], cu_seqlens_q[s+1]) of the packed q and out (none, one or
+ * many) and kv_lens[s] keys in its pages, the new tokens' included. Causal masking is bottom-right: new
+ * token i of n sees keys j <= i + kv_lens[s] - n. Keys on unmapped pages (ids < 0 or >= num_kv_blocks, or
+ * past max_blocks_per_seq) contribute nothing; a token that sees no key gives zeros and an lse of -inf.
+ * cu_seqlens_q, kv_lens and table_rows are HOST arrays, read during the call: the work is planned from
+ * them and travels in the kernels' arguments, so a captured launch replays with the lengths it was
+ * captured with. Rows of out and lse outside the sequences' tokens are left as they are.
+ * Pages are fp16 or bf16 (k_exp and v_exp NULL) or 8-bit (codes and exponent bytes of sca_kv8_layer;
+ * strides in bytes). */
+typedef struct sca_paged_varlen_params {
+    const void* q;                /* token t, head h at t*q_ss + h*q_sh */
+    const void* k;                /* layer base: pool row r, KV head h at r*k_ss + h*k_sh */
+    const void* v;
+    const uint8_t* k_exp;         /* exponent bytes of 8-bit pages, or NULL */
+    const uint8_t* v_exp;
+    void* out;                    /* token t, head h at t*o_ss + h*o_sh */
+    float* lse;                   /* optional FP32 [tokens, num_heads]; NULL = none */
+    const int32_t* page_table;    /* device, rows of max_blocks_per_seq entries */
+    const int32_t* cu_seqlens_q;  /* host, num_seqs + 1, non-decreasing */
+    const int32_t* kv_lens;       /* host, num_seqs */
+    const int32_t* table_rows;    /* host, num_seqs: the sequences' rows of page_table; NULL = 0, 1, ... */
+    int64_t num_seqs;
+    int64_t num_heads;
+    int64_t num_kv_heads;
+    int64_t head_dim;             /* 32, 64, 96, 128, 160, 192 or 256 */
+    int64_t block_size;           /* a power of two (8-bit pages: at least 8) */
+    int64_t max_blocks_per_seq;
+    int64_t num_kv_blocks;
+    int64_t q_ss, q_sh;
+    int64_t k_ss, k_sh;
+    int64_t v_ss, v_sh;
+    int64_t o_ss, o_sh;
+    float scale;                  /* softmax scale (already resolved, > 0) */
+    int32_t causal;
+    int32_t dtype;                /* SCA_DTYPE_F16 or SCA_DTYPE_BF16, of q, out and what the pages stand for */
+} sca_paged_varlen_params;
+
+/* Scratch that a run of these lengths wants (0: it would not split its keys, at most 64 MiB), and the
+ * run: with less scratch it splits less, with none not at all. The scratch is device memory, 16 B
+ * aligned, in use until the launches have completed on `stream`. The first reads no device pointer. */
+SCA_HIP_API int64_t sca_hip_paged_varlen_bytes(const sca_paged_varlen_params* params);
+SCA_HIP_API int sca_hip_paged_varlen(const sca_paged_varlen_params* params, void* scratch,
+                                     int64_t scratch_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------- */
 /* KV cache data movement over the block-major layout [num_blocks][block_size][H_kv][D]         */
 /* replaces: src/kv_cache/kv_cache_kernels.cuh:20-33 (LaunchKvAppend, LaunchKvResetBlock,       */
@@ -293,6 +354,33 @@ SCA_HIP_API int sca_hip_kv_reset_blocks(void* layer_k, void* layer_v, const int3
 SCA_HIP_API int sca_hip_kv_gather(const void* layer, const int32_t* block_ids,
                                   int64_t num_block_ids, void* out, const sca_kv_shape* shape,
                                   int64_t elem_bytes, void* stream);
+
+/* The same over pages that keep K and V in 8 bits (no reference counterpart). Codes are e4m3 bytes
+ * [num_blocks][block_size][H_kv][D]; every (token, head) row of K and of V has an exponent byte in
+ * [num_blocks][H_kv][block_size]: code c of a row with byte e stands for c * 2^(e - 127). A row whose
+ * largest magnitude is a is written with the least exponent that keeps a at or below 448 * 2^k (at
+ * least -126), its values rounded to the nearest code, ties to even. Magnitudes above 61440 (fp16) or
+ * 1.875 * 2^127 (bf16), infinities among them, are held as that value; NaN is held as NaN and does not
+ * count for a. Every value held is a number of the 16-bit type. Zeroed pages hold zeros.
+ * block_size is a multiple of 8, head_dim one of the seven attention head dims. */
+typedef struct sca_kv8_layer {
+    void* k;           /* codes, 16 B aligned */
+    void* v;
+    uint8_t* k_exp;    /* exponent bytes, 8 B aligned */
+    uint8_t* v_exp;
+} sca_kv8_layer;
+
+/* As sca_hip_kv_append; k_new/v_new are fp16 or bf16 [num_tokens, H_kv, D]. */
+SCA_HIP_API int sca_hip_kv8_append(const sca_kv8_layer* layer, const void* k_new, const void* v_new,
+                                   const int32_t* slot_mapping, int64_t num_tokens,
+                                   const sca_kv_shape* shape, int32_t dtype, void* stream);
+SCA_HIP_API int sca_hip_kv8_reset_blocks(const sca_kv8_layer* layer, const int32_t* block_ids,
+                                         int64_t num_block_ids, const sca_kv_shape* shape,
+                                         void* stream);
+/* out[i] <- the values of block block_ids[i], as fp16 or bf16 [n, block_size, H_kv, D]. */
+SCA_HIP_API int sca_hip_kv8_gather(const void* codes, const uint8_t* exponents,
+                                   const int32_t* block_ids, int64_t num_block_ids, void* out,
+                                   const sca_kv_shape* shape, int32_t dtype, void* stream);
 
 /* Sparse int32 update: dst[pairs[2i]] = pairs[2i+1] for i < num_pairs (indices outside
  * [0, dst_len) are skipped; pairs 8 B aligned, device). Used to refresh only the changed entries

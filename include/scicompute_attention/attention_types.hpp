@@ -16,6 +16,13 @@ enum class AttnLayout : int32_t { kBHSD = 0, kBSHD = 1 };
 // KV storage layout of KVCache: block-major [blocks][block_size][kv_heads][head_dim].
 enum class KvLayout : int32_t { kBlockMajor = 0 };
 
+// How a KV cache keeps its values:
+//   kSame = in the cache's dtype
+//   kE4M3 = in 8 bits, one e4m3 code a value and a power-of-two scale per (token, KV head) of K and of
+//           V (1 + 1/head_dim bytes a value); the cache's dtype, fp16 or bf16, is what goes in and what
+//           the codes stand for
+enum class KvStorage : int32_t { kSame = 0, kE4M3 = 1 };
+
 // Which implementation serves a request; kAuto lets the dispatcher decide.
 enum class BackendKind : int32_t {
     kAuto = 0,
@@ -52,6 +59,7 @@ SCI_ATTENTION_API int SupportedHeadDimIndex(int64_t head_dim) noexcept;
 SCI_ATTENTION_API const char* LayoutName(AttnLayout layout) noexcept;
 SCI_ATTENTION_API const char* BackendName(BackendKind kind) noexcept;
 SCI_ATTENTION_API const char* KvLayoutName(KvLayout layout) noexcept;
+SCI_ATTENTION_API const char* KvStorageName(KvStorage storage) noexcept;
 
 // FP32, FP16 and BF16 are the compute dtypes.
 SCI_ATTENTION_API bool IsSupportedComputeDtype(sci::DType dtype) noexcept;

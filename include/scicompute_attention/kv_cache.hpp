@@ -27,6 +27,7 @@ struct KVCacheConfig {
     sci::DType dtype{sci::DType::kFloat16};
     KvLayout layout{KvLayout::kBlockMajor};
     bool enable_stats{true};
+    KvStorage storage{KvStorage::kSame};  // kE4M3: pages of at least 8 tokens, fp16 or bf16 only
 };
 
 struct KVCacheStats {
@@ -43,6 +44,11 @@ struct KVCacheStats {
 //   [num_blocks][block_size][num_kv_heads][head_dim]
 // so a page is block_size * num_kv_heads * head_dim contiguous elements and one token row of a
 // page (all KV heads) is contiguous: the paged decode kernel reads it with 16-byte vector loads.
+// With KvStorage::kE4M3 those tensors hold one code byte a value (dtype kUInt8), and one exponent tensor
+// per layer for K and for V, [num_blocks][num_kv_heads][block_size] bytes, holds the rows' scales: code
+// c stands for c * 2^(e - 127). Append quantises, GatherK / GatherV give the values the codes stand for
+// (which the cache's dtype represents exactly), Reset leaves pages of zeros. Values above the largest
+// that 8 bits hold (61440 in fp16, 1.875 * 2^127 in bf16) are held as that; NaN stays NaN.
 class SCI_ATTENTION_API KVCache {
 public:
     KVCache() = default;
@@ -52,12 +58,13 @@ public:
     static sci::Result<KVCache> Create(const KVCacheConfig& cfg, sci::Device& device);
 
     // Scatters k_new/v_new [num_tokens, num_kv_heads, head_dim] (device) into the slots of
-    // `slot_mapping` (device int32, slot = page * block_size + offset; slot < 0 skips the token).
+    // `slot_mapping` (device int32, slot = page * block_size + offset; slot < 0 skips the token; the
+    // slots of one call are distinct).
     sci::Status Append(int64_t layer, const sci::Tensor& k_new, const sci::Tensor& v_new,
                        const int32_t* slot_mapping, int64_t num_tokens, sci::Stream* stream);
 
     // Copies the listed pages (device int32 ids) into a new [num_blocks, block_size, H_kv, D]
-    // tensor; ids outside the pool give zero pages. For tests and debugging.
+    // tensor of the cache's dtype; ids outside the pool give zero pages. For tests and debugging.
     sci::Result<sci::Tensor> GatherK(int64_t layer, const int32_t* block_ids, int64_t num_blocks,
                                      sci::Stream* stream) const;
     sci::Result<sci::Tensor> GatherV(int64_t layer, const int32_t* block_ids, int64_t num_blocks,
@@ -68,6 +75,9 @@ public:
 
     const sci::Tensor& K(int64_t layer) const;
     const sci::Tensor& V(int64_t layer) const;
+    // Exponent bytes of 8-bit storage (empty tensors otherwise).
+    const sci::Tensor& KExponents(int64_t layer) const;
+    const sci::Tensor& VExponents(int64_t layer) const;
     KVCacheStats Stats() const;
     size_t MemoryBytes() const noexcept;
     int64_t LayerElements() const noexcept { return layer_elements_; }
@@ -82,6 +92,8 @@ private:
     int64_t layer_elements_{0};
     std::vector<sci::Tensor> k_layers_;
     std::vector<sci::Tensor> v_layers_;
+    std::vector<sci::Tensor> k_exponents_;  // 8-bit storage
+    std::vector<sci::Tensor> v_exponents_;
     KVCacheStats stats_{};
 };
 
@@ -91,7 +103,8 @@ SCI_ATTENTION_API sci::Result<std::vector<int32_t>> ComputeSlotMapping(
     const int32_t* block_table_row, int64_t seq_start, int64_t num_tokens, int64_t block_size,
     int64_t max_blocks);
 
-// 2 * num_layers * num_blocks * block_size * num_kv_heads * head_dim * sizeof(dtype).
+// 2 * num_layers * num_blocks * block_size * num_kv_heads * head_dim * sizeof(dtype); with 8-bit storage
+// (head_dim + 1) bytes in the place of head_dim * sizeof(dtype).
 SCI_ATTENTION_API sci::Result<size_t> KvCacheBytes(const KVCacheConfig& cfg);
 
 // floor(budget_bytes / bytes per page across K, V and all layers); 0 when a page does not fit.

@@ -1,0 +1,322 @@
+// The general kernel of attention over paged KV (paged_varlen.hpp): every head_dim, 16-bit and 8-bit
+// pages.
+//
+// Four waves of 32 packed rows; key tiles of 64 keys (32 from head_dim 160 on) come through registers
+// into two LDS buffers: while a tile is multiplied the next one's loads are in flight, and 8-bit codes
+// are widened (e4m3.hpp) on their way into LDS, so that one inner loop serves both kinds of pages. A
+// lane looks up the page of one key per tile, one tile ahead of the loads that need it, and hands the
+// row to the lanes that copy it with a shuffle. Formulation, swizzles and online softmax are those of
+// the flash kernels (flash_common.hpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "e4m3.hpp"
+#include "paged_varlen.hpp"
+
+namespace sca_hip {
+namespace {
+
+template <int D, bool kHeld8>
+struct TileGeom {
+    static constexpr int BN = D <= 128 ? 64 : 32;      // keys per tile
+    static constexpr int NT = BN / 32;                 // S^T tiles of 32 keys
+    static constexpr int KS = D / 16;
+    static constexpr int DT = D / 32;
+    static constexpr int RB = 2 * D;                   // LDS row bytes
+    static constexpr int TILE_BYTES = BN * RB;
+    static constexpr int CPR = kHeld8 ? D / 16 : D / 8;  // 16-byte chunks of a row in memory
+    static constexpr int CHUNKS = BN * CPR;
+    static constexpr int PER = (CHUNKS + 255) / 256;   // chunks per thread
+    static constexpr int LDS_BYTES = 4 * TILE_BYTES;   // two buffers of K and V
+    static_assert(CHUNKS % kWave == 0, "a wave copies a chunk on all lanes or on none (shuffles)");
+    static constexpr int WG_PER_CU = D <= 128 ? 2 : 1;
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (a plain vector stays in registers)
+
+__device__ __forceinline__ u32x4 Masked(const u32x4& w, uint32_t keep) { return w & keep; }
+
+// log2 headroom of the weights: they are 2^(x - mu) with mu that much below the row's maximum. fp16
+// weights then keep all their bits down to 2^-21 of the largest (2^-14 without), and stay finite: at
+// most 2^(7 + kRescaleSlack).
+template <typename E>
+struct WeightBias {
+    static constexpr float value = 0.0f;
+};
+template <>
+struct WeightBias<F16> {
+    static constexpr float value = 7.0f;
+};
+
+template <typename E, int D, bool kHeld8>
+__global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_tile_kernel(
+    const PagedArgs p, const PagedSeqs seqs) {
+    using G = TileGeom<D, kHeld8>;
+    using M = Mfma<E>;
+    using vec8 = typename E::vec8;
+    constexpr int BN = G::BN;
+    constexpr float kBias = WeightBias<E>::value;
+
+    extern __shared__ __align__(16) uint8_t lds8[];
+    uint8_t* lds_k = lds8;
+    uint8_t* lds_v = lds8 + 2 * G::TILE_BYTES;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int lane = tid % kWave;
+    const int lr = lane & 31;
+    const int hh = lane >> 5;
+
+    const PagedUnit u = FindUnit(seqs, p.kv_heads);
+    const PagedSeq& sq = u.seq;
+    const int rows = sq.q_count * p.group;
+    const int diag = p.causal ? sq.keys - sq.q_count : 0;
+    const int visible = VisibleKeys(sq, u.tile, p.group, p.causal != 0);
+    const int all_tiles = (visible + BN - 1) / BN;
+    int first = 0, n_tiles = all_tiles;
+    if (sq.splits > 1) SplitRange(all_tiles, sq.splits, u.split, &first, &n_tiles);
+
+    // This lane's row, its token and head; rows past the last one repeat it and are not stored.
+    const int row = u.tile * kPagedRows + 32 * wave + lr;
+    const bool row_ok = row < rows;
+    const int safe_row = min(row, rows - 1);
+    const int token = static_cast<int>(static_cast<uint32_t>(safe_row) / static_cast<uint32_t>(p.group));
+    const int head = u.h_kv * p.group + safe_row - token * p.group;
+    const int limit = p.causal ? min(sq.keys - 1, token + diag) : sq.keys - 1;  // last visible key
+    // The wave's least limit: tiles that end at or before it need no mask for it.
+    const int wave_row = min(u.tile * kPagedRows + 32 * wave, rows - 1);
+    const int wave_limit =
+        p.causal ? min(sq.keys - 1, static_cast<int>(static_cast<uint32_t>(wave_row) /
+                                                     static_cast<uint32_t>(p.group)) + diag)
+                 : sq.keys - 1;
+
+    vec8 qf[G::KS];
+    {
+        const uint16_t* q_row = static_cast<const uint16_t*>(p.q) +
+                                static_cast<int64_t>(sq.q_first + token) * p.q_ss + head * p.q_sh + 8 * hh;
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks) {
+            qf[ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const uint4*>(q_row + 16 * ks));
+        }
+    }
+
+    constexpr int kEb = kHeld8 ? 1 : 2;
+    const uint8_t* k_base = static_cast<const uint8_t*>(p.k) + u.h_kv * p.k_sh * kEb;
+    const uint8_t* v_base = static_cast<const uint8_t*>(p.v) + u.h_kv * p.v_sh * kEb;
+    const int64_t k_row_bytes = p.k_ss * kEb;
+    const int64_t v_row_bytes = p.v_ss * kEb;
+    const int32_t* table = p.page_table + static_cast<int64_t>(sq.table_row) * p.max_blocks;
+    const int bs_mask = (1 << p.block_shift) - 1;
+
+    // Pool row of key lane % BN of tile t, or -1 (past the keys, unmapped, outside the pool).
+    auto row_of = [&](int t) __attribute__((always_inline)) -> int {
+        const int key = t * BN + lane % BN;
+        const int logical = key >> p.block_shift;
+        if (t >= first + n_tiles || key >= sq.keys || logical >= p.max_blocks) return -1;
+        const int32_t id = table[logical];
+        if (id < 0 || id >= p.num_blocks) return -1;
+        return (id << p.block_shift) | (key & bs_mask);
+    };
+    u32x4 kr[G::PER], vr[G::PER];
+    uint32_t k_byte = 0, v_byte = 0;  // exponent bytes of key lane % BN
+    uint64_t valid = 0;               // keys of the tile in flight that exist (bit per key)
+    auto issue = [&](int pool_row) __attribute__((always_inline)) {
+        valid = __builtin_amdgcn_ballot_w64(pool_row >= 0);
+        const int safe = pool_row < 0 ? 0 : pool_row;
+        if constexpr (kHeld8) {
+            const int64_t at = ((static_cast<int64_t>(safe >> p.block_shift) * p.kv_heads + u.h_kv)
+                                << p.block_shift) + (safe & bs_mask);
+            k_byte = p.k_exp[at];
+            v_byte = p.v_exp[at];
+        }
+#pragma unroll
+        for (int i = 0; i < G::PER; ++i) {
+            const int c = i * 256 + tid;
+            if (G::CHUNKS % 256 != 0 && c >= G::CHUNKS) continue;
+            const int64_t r = __shfl(safe, c / G::CPR);
+            kr[i] = *reinterpret_cast<const u32x4*>(k_base + r * k_row_bytes + (c % G::CPR) * 16);
+            vr[i] = *reinterpret_cast<const u32x4*>(v_base + r * v_row_bytes + (c % G::CPR) * 16);
+        }
+    };
+    // Registers -> LDS buffer `buf`. V rows of keys that do not exist are cleared: their weights are
+    // zero, but the row may hold a NaN.
+    auto Widen = [](uint32_t lo, uint32_t hi, float unit) __attribute__((always_inline)) {
+        return __builtin_bit_cast(u32x4, Widen8<E>(lo, hi, unit));
+    };
+    auto put = [&](int buf) __attribute__((always_inline)) {
+        uint8_t* dk = lds_k + buf * G::TILE_BYTES;
+        uint8_t* dv = lds_v + buf * G::TILE_BYTES;
+#pragma unroll
+        for (int i = 0; i < G::PER; ++i) {
+            const int c = i * 256 + tid;
+            if (G::CHUNKS % 256 != 0 && c >= G::CHUNKS) continue;
+            const int r = c / G::CPR;
+            const int pos = c % G::CPR;
+            const uint32_t keep = (valid >> r) & 1 ? ~0u : 0u;
+            if constexpr (kHeld8) {
+                const float ku = UnitOf(__shfl(k_byte, r)), vu = UnitOf(__shfl(v_byte, r));
+                const u32x4 k0 = Widen(kr[i].x, kr[i].y, ku), k1 = Widen(kr[i].z, kr[i].w, ku);
+                const u32x4 v0 = Widen(vr[i].x, vr[i].y, vu), v1 = Widen(vr[i].z, vr[i].w, vu);
+                *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos) ^ SwzK<D>(r)) * 16)) = k0;
+                *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos + 1) ^ SwzK<D>(r)) * 16)) = k1;
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos) ^ SwzV<D>(r)) * 16)) = Masked(v0, keep);
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos + 1) ^ SwzV<D>(r)) * 16)) = Masked(v1, keep);
+            } else {
+                *reinterpret_cast<u32x4*>(dk + r * G::RB + ((pos ^ SwzK<D>(r)) * 16)) = kr[i];
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + ((pos ^ SwzV<D>(r)) * 16)) = Masked(vr[i], keep);
+            }
+        }
+    };
+
+    floatx16 o[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+    }
+    float mu = neg_inf();  // reference point of the weights (log2 units)
+    float l = 0.0f;        // this lane's share of the denominator
+    const float scale2 = p.scale * kLog2e;
+
+    // Fragment positions (flash_common.hpp).
+    const int grp = lane >> 4;
+    const int sl = lane & 15;
+    const int v_key = 4 * hh + (sl >> 2);
+    const int v_chunk = 2 * (grp & 1) + ((sl & 3) >> 1);
+    const int v_half = (sl & 1) * 8;
+
+    auto compute = [&](int buf, int t, uint64_t keys_ok) __attribute__((always_inline)) {
+        const uint8_t* sk = lds_k + buf * G::TILE_BYTES;
+        const uint8_t* sv = lds_v + buf * G::TILE_BYTES;
+        floatx16 s[G::NT];
+#pragma unroll
+        for (int n = 0; n < G::NT; ++n) {
+            const int kr_ = 32 * n + lr;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks) {
+                const uint4 f = *reinterpret_cast<const uint4*>(sk + kr_ * G::RB +
+                                                                (((2 * ks + hh) ^ SwzK<D>(kr_)) * 16));
+                s[n] = M::mma(__builtin_bit_cast(vec8, f), qf[ks], s[n]);
+            }
+        }
+        if (keys_ok != ~uint64_t{0} || t * BN + BN - 1 > wave_limit) {
+            const int base = t * BN + 4 * hh;
+#pragma unroll
+            for (int n = 0; n < G::NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int k_in = 32 * n + 8 * (i / 4) + (i % 4);
+                    const bool seen = base + k_in <= limit && ((keys_ok >> (k_in + 4 * hh)) & 1);
+                    s[n][i] = seen ? s[n][i] : neg_inf();
+                }
+            }
+        }
+        float mx = Max16(s[0]);
+        if constexpr (G::NT > 1) mx = fmaxf(mx, Max16(s[G::NT - 1]));
+        const float top = HalfMax(mx) * scale2;
+        if (__builtin_amdgcn_ballot_w64(top > mu + kBias + kRescaleSlack) != 0) {
+            const bool grow = top > mu + kBias + kRescaleSlack;
+            const float mu_new = grow ? top - kBias : mu;
+            const float alpha = grow ? fast_exp2(mu - mu_new) : 1.0f;  // 0 where mu was -inf
+            mu = mu_new;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < G::DT; ++dt) o[dt] *= alpha;
+        }
+        const float neg_mu = mu == neg_inf() ? 0.0f : -mu;
+        vec8 pb[2 * G::NT];
+#pragma unroll
+        for (int n = 0; n < G::NT; ++n) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float a = fast_exp2(fmaf(s[n][2 * i], scale2, neg_mu));
+                const float b = fast_exp2(fmaf(s[n][2 * i + 1], scale2, neg_mu));
+                l += a + b;
+                // Rounded once to the 16-bit type, by at most half a step, as the output is.
+                w[i] = M::pack(a, b);
+            }
+            pb[2 * n] = __builtin_bit_cast(vec8, make_uint4(w[0], w[1], w[2], w[3]));
+            pb[2 * n + 1] = __builtin_bit_cast(vec8, make_uint4(w[4], w[5], w[6], w[7]));
+        }
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt) {
+#pragma unroll
+            for (int n = 0; n < G::NT; ++n) {
+                const uint8_t* a = sv + (32 * n + v_key) * G::RB +
+                                   (((4 * dt + v_chunk) ^ SwzV<D>(v_key)) * 16) + v_half;
+#pragma unroll
+                for (int ps = 0; ps < 2; ++ps) {
+                    const uint2 lo = TrRead<E>::read(a + (16 * ps) * G::RB);
+                    const uint2 hi = TrRead<E>::read(a + (16 * ps + 8) * G::RB);
+                    o[dt] = M::mma(__builtin_bit_cast(vec8, make_uint4(lo.x, lo.y, hi.x, hi.y)),
+                                   pb[2 * n + ps], o[dt]);
+                }
+            }
+        }
+    };
+
+    if (n_tiles > 0) {
+        issue(row_of(first));
+        int next = row_of(first + 1);
+        put(0);
+        uint64_t now_ok = valid;
+        __syncthreads();
+        for (int j = 0; j < n_tiles; ++j) {
+            const bool more = j + 1 < n_tiles;
+            if (more) {
+                issue(next);
+                next = row_of(first + j + 2);
+            }
+            compute(j & 1, first + j, now_ok);
+            if (more) {
+                put((j + 1) & 1);
+                now_ok = valid;
+            }
+            __syncthreads();
+        }
+    }
+
+    const float l_all = HalfSum(l);
+    if (sq.splits > 1) {
+        const int64_t state = sq.state_base + (static_cast<int64_t>(u.split) * p.kv_heads + u.h_kv) * rows + row;
+        if (row_ok && hh == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * state) = make_float2(mu, l_all);
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt) {
+            float a[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a[i] = o[dt][i];
+            StorePartialTile(p.part_o + state * D + 32 * dt, hh, row_ok, a);
+        }
+        return;
+    }
+    const float inv = l_all > 0.0f ? 1.0f / l_all : l_all;  // (NaN stays NaN)
+    uint16_t* out_row = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(sq.q_first + token) * p.o_ss +
+                        head * p.o_sh;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt) {
+        float a[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a[i] = o[dt][i] * inv;
+        StoreTile<M>(out_row + 32 * dt, hh, row_ok, a);
+    }
+    if (p.lse != nullptr && row_ok && hh == 0) {
+        p.lse[static_cast<int64_t>(sq.q_first + token) * p.heads + head] =
+            l_all == 0.0f ? neg_inf() : (mu + __log2f(l_all)) * kLn2;
+    }
+}
+
+}  // namespace
+
+template <typename E, int D, bool kHeld8>
+int LaunchPagedTile(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s) {
+    using G = TileGeom<D, kHeld8>;
+    if (const int rc = EnsureLdsLimit<&paged_tile_kernel<E, D, kHeld8>>(G::LDS_BYTES, "paged LDS limit")) return rc;
+    hipLaunchKernelGGL((paged_tile_kernel<E, D, kHeld8>), dim3(static_cast<unsigned>(units)), dim3(256),
+                       G::LDS_BYTES, s, a, seqs);
+    return CheckLaunch("paged_tile_kernel", s);
+}
+
+}  // namespace sca_hip

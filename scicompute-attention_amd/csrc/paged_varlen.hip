@@ -1,0 +1,322 @@
+// Attention of ragged chunks of new tokens over paged KV: the plan of a call (units, key splits, the
+// launches' sequence lists), the merge of key splits, the checks and the C entry points. The kernels
+// are in paged_tile.hpp; paged_varlen.hpp describes rows, units and splits.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <exception>
+#include <string>
+#include <vector>
+
+#include "paged_varlen.hpp"
+
+namespace sca_hip {
+namespace {
+
+constexpr int kCombineThreads = 256;
+constexpr int64_t kMostScratch = int64_t{64} << 20;
+
+// out = sum_s O_s 2^(mu_s - mu*) / sum_s l_s 2^(mu_s - mu*), one thread per (row, 4 dims); grid.y is
+// the sequence. A range that saw no key has l = 0 and counts for nothing.
+template <typename E>
+__global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(const PagedArgs p,
+                                                                        const PagedSeqs seqs,
+                                                                        uint32_t head_dim) {
+    using M = Mfma<E>;
+    const PagedSeq sq = seqs.seq[blockIdx.y];
+    if (sq.splits <= 1) return;
+    const uint32_t rows = static_cast<uint32_t>(sq.q_count) * static_cast<uint32_t>(p.group);
+    const uint32_t all = rows * static_cast<uint32_t>(p.kv_heads);
+    const uint32_t quads = head_dim / 4;
+    const uint32_t idx = blockIdx.x * kCombineThreads + threadIdx.x;
+    const uint32_t at = idx / quads;  // (KV head, packed row)
+    if (at >= all) return;
+    const uint32_t d0 = (idx - at * quads) * 4;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + sq.state_base + at;
+    const float* po = p.part_o + (static_cast<int64_t>(sq.state_base) + at) * head_dim + d0;
+    float mu = neg_inf();
+#pragma unroll 4
+    for (int s = 0; s < sq.splits; ++s) mu = fmaxf(mu, ml[static_cast<int64_t>(s) * all].x);
+    float l = 0.0f;
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < sq.splits; ++s) {
+        const float2 st = ml[static_cast<int64_t>(s) * all];
+        if (st.y == 0.0f) continue;
+        // (a range whose scores were all NaN has no maximum but a NaN sum, which must stay)
+        const float w = st.x == neg_inf() ? 1.0f : fast_exp2(st.x - mu);
+        l = fmaf(st.y, w, l);
+        const float4 v = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * all * head_dim);
+        a[0] = fmaf(v.x, w, a[0]);
+        a[1] = fmaf(v.y, w, a[1]);
+        a[2] = fmaf(v.z, w, a[2]);
+        a[3] = fmaf(v.w, w, a[3]);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    const uint32_t h_kv = at / rows;
+    const uint32_t row = at - h_kv * rows;
+    const uint32_t token = row / static_cast<uint32_t>(p.group);
+    const int64_t head = h_kv * p.group + (row - token * p.group);
+    const int64_t out_row = static_cast<int64_t>(sq.q_first) + token;
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out_row * p.o_ss + head * p.o_sh + d0) =
+        make_uint2(M::pack(a[0] * inv, a[1] * inv), M::pack(a[2] * inv, a[3] * inv));
+    if (p.lse != nullptr && d0 == 0) {
+        p.lse[out_row * p.heads + head] = l == 0.0f ? neg_inf() : (mu + __log2f(l)) * kLn2;
+    }
+}
+
+bool Aligned(const void* ptr, uintptr_t bytes) {
+    return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0;
+}
+
+int KeysPerTile(int64_t head_dim) { return head_dim <= 128 ? 64 : 32; }
+
+// One sequence of a call, in the order of the launches.
+struct Planned {
+    PagedSeq seq;
+    int64_t tiles;  // key tiles of its last row tile
+};
+
+struct Plan {
+    std::vector<PagedSeqs> launches;
+    std::vector<int64_t> units;
+    std::vector<int64_t> combine_rows;  // most (KV head, row) pairs of a split sequence; 0: no merge
+    int64_t states = 0;                 // most states a launch leaves
+};
+
+// Workgroups that the GPU holds at once.
+int64_t Resident(int64_t head_dim) {
+    return static_cast<int64_t>(CuCount()) * (head_dim <= 96 ? 2 : 1);
+}
+
+// `may_split`: states may go to `most_states` of scratch.
+Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
+    const int64_t group = p.num_heads / p.num_kv_heads;
+    const int bn = KeysPerTile(p.head_dim);
+    std::vector<Planned> list;
+    int64_t work = 0;   // key tiles of all units
+    for (int64_t s = 0; s < p.num_seqs; ++s) {
+        const int64_t n = p.cu_seqlens_q[s + 1] - p.cu_seqlens_q[s];
+        if (n == 0) continue;
+        Planned e{};
+        e.seq.q_first = p.cu_seqlens_q[s];
+        e.seq.q_count = static_cast<int32_t>(n);
+        e.seq.keys = p.kv_lens[s];
+        e.seq.table_row = p.table_rows != nullptr ? p.table_rows[s] : static_cast<int32_t>(s);
+        e.seq.splits = 1;
+        e.seq.row_tiles = static_cast<int32_t>((n * group + kPagedRows - 1) / kPagedRows);
+        e.tiles = (p.kv_lens[s] + bn - 1) / bn;
+        // (causal: the row tiles of new tokens see fewer keys; their mean serves the estimate)
+        const int64_t mean = p.causal ? std::max<int64_t>(1, e.tiles - std::min<int64_t>(n, p.kv_lens[s]) / (2 * bn))
+                                      : e.tiles;
+        work += p.num_kv_heads * e.seq.row_tiles * mean;
+        list.push_back(e);
+    }
+    // Key splits: every unit at most the share of one resident workgroup (and at least kLeastTiles), for
+    // the sequences where that saves kWorthTiles steps of the longest unit: the states' traffic and the
+    // merge's launch cost about as much as those.
+    constexpr int64_t kLeastTiles = 4, kWorthTiles = 8;
+    const int64_t span = std::max<int64_t>(kLeastTiles, (work + Resident(p.head_dim) - 1) / Resident(p.head_dim));
+    for (Planned& e : list) {
+        if (most_states > 0 && e.tiles - span >= kWorthTiles) {
+            e.seq.splits = static_cast<int32_t>(std::min<int64_t>(64, (e.tiles + span - 1) / span));
+        }
+    }
+    // Longest units first.
+    std::stable_sort(list.begin(), list.end(), [](const Planned& a, const Planned& b) {
+        return a.tiles * b.seq.splits > b.tiles * a.seq.splits;
+    });
+    Plan plan;
+    for (size_t at = 0; at < list.size(); at += kPagedSeqs) {
+        PagedSeqs seqs{};
+        int64_t units = 0, states = 0, combine = 0;
+        for (size_t i = at; i < std::min(list.size(), at + kPagedSeqs); ++i) {
+            PagedSeq q = list[i].seq;
+            const int64_t rows = q.q_count * group * p.num_kv_heads;
+            while (q.splits > 1 && states + rows * q.splits > most_states) --q.splits;
+            q.state_base = static_cast<int32_t>(states);
+            if (q.splits > 1) {
+                states += rows * q.splits;
+                combine = std::max(combine, rows);
+            }
+            units += static_cast<int64_t>(q.row_tiles) * q.splits * p.num_kv_heads;
+            q.unit_end = static_cast<int32_t>(std::min<int64_t>(units, 0x7fffffff));
+            seqs.seq[seqs.count++] = q;
+        }
+        plan.launches.push_back(seqs);
+        plan.units.push_back(units);
+        plan.combine_rows.push_back(combine);
+        plan.states = std::max(plan.states, states);
+    }
+    return plan;
+}
+
+int64_t StateBytes(int64_t head_dim) { return 4 * (head_dim + 2); }
+
+template <typename E>
+int LaunchTile(const PagedArgs& a, const PagedSeqs& seqs, int units, int64_t head_dim, hipStream_t s) {
+    const bool held8 = a.k_exp != nullptr;
+    switch (head_dim) {
+#define SCA_CASE(D) \
+    case D: return held8 ? LaunchPagedTile<E, D, true>(a, seqs, units, s) : LaunchPagedTile<E, D, false>(a, seqs, units, s);
+        SCA_CASE(32)
+        SCA_CASE(64)
+        SCA_CASE(96)
+        SCA_CASE(128)
+        SCA_CASE(160)
+        SCA_CASE(192)
+        SCA_CASE(256)
+#undef SCA_CASE
+        default: break;
+    }
+    return SetError(SCA_E_UNSUPPORTED_HEAD_DIM,
+                    "paged varlen: head_dim=" + std::to_string(head_dim) + " is not instantiated");
+}
+
+template <typename E>
+int Run(const sca_paged_varlen_params& p, const Plan& plan, void* scratch, hipStream_t s) {
+    PagedArgs a{};
+    a.q = p.q, a.k = p.k, a.v = p.v, a.k_exp = p.k_exp, a.v_exp = p.v_exp;
+    a.out = p.out, a.lse = p.lse, a.page_table = p.page_table;
+    a.part_o = static_cast<float*>(scratch);
+    a.part_ml = a.part_o + plan.states * p.head_dim;
+    a.max_blocks = p.max_blocks_per_seq, a.num_blocks = p.num_kv_blocks;
+    a.q_ss = p.q_ss, a.q_sh = p.q_sh, a.k_ss = p.k_ss, a.k_sh = p.k_sh;
+    a.v_ss = p.v_ss, a.v_sh = p.v_sh, a.o_ss = p.o_ss, a.o_sh = p.o_sh;
+    a.heads = static_cast<int32_t>(p.num_heads);
+    a.kv_heads = static_cast<int32_t>(p.num_kv_heads);
+    a.group = static_cast<int32_t>(p.num_heads / p.num_kv_heads);
+    while ((int64_t{1} << a.block_shift) < p.block_size) ++a.block_shift;
+    a.causal = p.causal;
+    a.scale = p.scale;
+    for (size_t i = 0; i < plan.launches.size(); ++i) {
+        int rc = LaunchTile<E>(a, plan.launches[i], static_cast<int>(plan.units[i]), p.head_dim, s);
+        if (rc != 0) return rc;
+        if (plan.combine_rows[i] == 0) continue;
+        const int64_t threads = plan.combine_rows[i] * (p.head_dim / 4);
+        const dim3 grid(static_cast<unsigned>((threads + kCombineThreads - 1) / kCombineThreads),
+                        static_cast<unsigned>(plan.launches[i].count));
+        hipLaunchKernelGGL((paged_combine_kernel<E>), grid, dim3(kCombineThreads), 0, s, a, plan.launches[i],
+                           static_cast<uint32_t>(p.head_dim));
+        rc = CheckLaunch("paged_combine_kernel", s);
+        if (rc != 0) return rc;
+    }
+    return 0;
+}
+
+// Everything that can be checked without the pointers' targets; `pointers` false leaves those out.
+int Validate(const sca_paged_varlen_params* p, bool pointers) {
+    auto fail = [](int code, const std::string& what) { return SetError(code, "paged varlen: " + what); };
+    if (p == nullptr) return fail(SCA_E_SHAPE_MISMATCH, "null params");
+    if (p->cu_seqlens_q == nullptr || p->kv_lens == nullptr) {
+        return fail(SCA_E_SHAPE_MISMATCH, "null cu_seqlens_q or kv_lens (host arrays)");
+    }
+    if (pointers) {
+        if (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr ||
+            p->page_table == nullptr) {
+            return fail(SCA_E_SHAPE_MISMATCH, "null pointer");
+        }
+        if ((p->k_exp == nullptr) != (p->v_exp == nullptr)) {
+            return fail(SCA_E_SHAPE_MISMATCH, "k_exp and v_exp must both be set (8-bit pages) or both NULL");
+        }
+        if (!Aligned(p->q, 16) || !Aligned(p->k, 16) || !Aligned(p->v, 16) || !Aligned(p->out, 16)) {
+            return fail(SCA_E_LAYOUT_MISMATCH, "q, k, v and out must be 16 B aligned");
+        }
+    }
+    if (p->num_seqs < 1 || p->num_seqs > 0x7fffffffLL / 2) {
+        return fail(SCA_E_SHAPE_MISMATCH, "num_seqs=" + std::to_string(p->num_seqs));
+    }
+    if (p->num_heads < 1 || p->num_heads > 65535 || p->num_kv_heads < 1 || p->num_heads % p->num_kv_heads != 0) {
+        return fail(SCA_E_SHAPE_MISMATCH, "invalid heads (H_q=" + std::to_string(p->num_heads) +
+                                              ", H_kv=" + std::to_string(p->num_kv_heads) + ")");
+    }
+    if (p->head_dim % 32 != 0 || p->head_dim < 32 || p->head_dim > 256 || p->head_dim == 224) {
+        return fail(SCA_E_UNSUPPORTED_HEAD_DIM, "head_dim=" + std::to_string(p->head_dim));
+    }
+    if (p->dtype != SCA_DTYPE_F16 && p->dtype != SCA_DTYPE_BF16) {
+        return fail(SCA_E_UNSUPPORTED_DTYPE, "computes in fp16/bf16; dtype id " + std::to_string(p->dtype));
+    }
+    if (!(p->scale > 0.0f) || p->scale > 3.0e38f) {
+        return fail(SCA_E_SHAPE_MISMATCH, "scale must be positive and finite");
+    }
+    const int64_t bs = p->block_size;
+    if (bs < 1 || (bs & (bs - 1)) != 0 || p->max_blocks_per_seq < 1 || p->num_kv_blocks < 1 ||
+        p->num_kv_blocks > 0x7fffffffLL / bs) {
+        return fail(SCA_E_SHAPE_MISMATCH,
+                    "block_size must be a power of two, max_blocks_per_seq and num_kv_blocks positive, and the "
+                    "pool's tokens below 2^31");
+    }
+    const bool held8 = p->k_exp != nullptr;
+    if (held8 && bs < 8) return fail(SCA_E_SHAPE_MISMATCH, "8-bit pages hold at least 8 tokens");
+    const int64_t ve = held8 ? 16 : 8;
+    if (p->q_ss % 8 || p->q_sh % 8 || p->o_ss % 8 || p->o_sh % 8 || p->k_ss % ve || p->k_sh % ve ||
+        p->v_ss % ve || p->v_sh % ve) {
+        return fail(SCA_E_LAYOUT_MISMATCH, "strides must be multiples of 16 B");
+    }
+    const int64_t group = p->num_heads / p->num_kv_heads;
+    int64_t units = 0;
+    if (p->cu_seqlens_q[0] < 0) return fail(SCA_E_SHAPE_MISMATCH, "cu_seqlens_q starts below 0");
+    for (int64_t s = 0; s < p->num_seqs; ++s) {
+        const int64_t n = static_cast<int64_t>(p->cu_seqlens_q[s + 1]) - p->cu_seqlens_q[s];
+        if (n < 0) {
+            return fail(SCA_E_SHAPE_MISMATCH, "cu_seqlens_q decreases at sequence " + std::to_string(s));
+        }
+        if (p->kv_lens[s] < 0) {
+            return fail(SCA_E_SHAPE_MISMATCH, "kv_lens[" + std::to_string(s) + "]=" + std::to_string(p->kv_lens[s]));
+        }
+        if (p->table_rows != nullptr && p->table_rows[s] < 0) {
+            return fail(SCA_E_SHAPE_MISMATCH, "table_rows[" + std::to_string(s) + "] is negative");
+        }
+        // Keys, and a sequence's rows over its KV heads, are 32-bit numbers in the kernels (with room
+        // for a tile past the end).
+        if (p->kv_lens[s] > 0x7fffffff - 4096 || n > 0x7fffffffLL / (p->num_heads * (p->head_dim / 4)) - kPagedRows) {
+            return fail(SCA_E_SEQ_TOO_LONG, "sequence " + std::to_string(s) + " of " + std::to_string(n) +
+                                                " new tokens and " + std::to_string(p->kv_lens[s]) + " keys");
+        }
+        units += (n * group + kPagedRows - 1) / kPagedRows * p->num_kv_heads;
+    }
+    if (units > 0x7fffffffLL / 64) {
+        return fail(SCA_E_SEQ_TOO_LONG, "grid of " + std::to_string(units) + " row tiles exceeds the launch limit");
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace sca_hip
+
+using sca_hip::SetError;
+
+extern "C" {
+
+int64_t sca_hip_paged_varlen_bytes(const sca_paged_varlen_params* params) {
+    if (sca_hip::Validate(params, /*pointers=*/false) != 0) return 0;
+    try {
+        const int64_t state = sca_hip::StateBytes(params->head_dim);
+        return sca_hip::MakePlan(*params, sca_hip::kMostScratch / state).states * state;
+    } catch (const std::exception&) {  // no host memory for the plan: the run will say so
+        return 0;
+    }
+}
+
+int sca_hip_paged_varlen(const sca_paged_varlen_params* params, void* scratch, int64_t scratch_bytes,
+                         void* stream) {
+    if (const int rc = sca_hip::Validate(params, /*pointers=*/true)) return rc;
+    if (!sca_hip::Aligned(scratch, 16)) {
+        return SetError(SCA_E_LAYOUT_MISMATCH, "paged varlen: scratch must be 16 B aligned");
+    }
+    const int64_t state = sca_hip::StateBytes(params->head_dim);
+    const int64_t room = scratch != nullptr && scratch_bytes > 0
+                             ? std::min(scratch_bytes, sca_hip::kMostScratch) / state
+                             : 0;
+    try {
+        const sca_hip::Plan plan = sca_hip::MakePlan(*params, room);
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        return params->dtype == SCA_DTYPE_F16 ? sca_hip::Run<sca_hip::F16>(*params, plan, scratch, s)
+                                              : sca_hip::Run<sca_hip::BF16>(*params, plan, scratch, s);
+    } catch (const std::exception& e) {
+        return SetError(SCA_E_WORKSPACE, std::string("paged varlen: no host memory for the plan: ") + e.what());
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,106 @@
+// Attention of ragged chunks of new tokens over paged KV: what the kernels and their plan share.
+//
+// Rows. The query heads of one KV head read the same keys, so their rows share row tiles: packed row
+// R of a (sequence, KV head) is new token R / group of head R % group. A chunk of 32 tokens with four
+// heads a group is one 128-row tile; a single token fills `group` rows of its tile.
+// Units. A workgroup takes one unit: (sequence, row tile, key split, KV head). The sequences of a
+// launch are listed in the kernel's arguments (PagedSeq), at most kPagedSeqs of them; more go out in
+// further launches. So nothing is uploaded, and a captured launch keeps its own list.
+// Splits. Where few row tiles meet many keys, a tile's keys are cut into ranges of whole key tiles,
+// and every range leaves the unnormalised fp32 state of its rows (O, reference point mu in log2
+// units, l) in scratch for paged_combine_kernel.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "flash_common.hpp"
+#include "sca_device.hpp"
+
+namespace sca_hip {
+
+constexpr int kPagedRows = 128;   // packed rows per workgroup
+constexpr int kPagedSeqs = 112;   // sequences per launch: 32 B each, below 4 KB of arguments
+
+struct PagedSeq {
+    int32_t unit_end;    // units of this and all earlier sequences of the launch
+    int32_t q_first;     // first new token's row in q and out
+    int32_t q_count;     // new tokens
+    int32_t keys;        // keys, the new tokens' included
+    int32_t table_row;   // row of the page table
+    int32_t splits;      // key splits of its row tiles
+    int32_t state_base;  // its first state in scratch (splits > 1)
+    int32_t row_tiles;
+};
+
+struct PagedSeqs {
+    int32_t count;
+    int32_t reserved;
+    PagedSeq seq[kPagedSeqs];
+};
+
+struct PagedArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const uint8_t* k_exp;  // 8-bit pages
+    const uint8_t* v_exp;
+    void* out;
+    float* lse;
+    const int32_t* page_table;
+    float* part_o;   // [state][D]
+    float* part_ml;  // [state][2]
+    int64_t max_blocks, num_blocks;
+    int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh, o_ss, o_sh;
+    int32_t heads, kv_heads, group, block_shift, causal;
+    float scale;
+};
+static_assert(sizeof(PagedArgs) + sizeof(PagedSeqs) <= 4096, "kernel arguments");
+
+// Launchers, instantiated in the file of their kernel; `units` workgroups.
+template <typename E, int D, bool kHeld8>
+int LaunchPagedTile(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_tile.hpp
+
+namespace {
+
+// The unit of this workgroup.
+struct PagedUnit {
+    PagedSeq seq;
+    int tile, split, h_kv;
+};
+
+__device__ __forceinline__ PagedUnit FindUnit(const PagedSeqs& seqs, int kv_heads) {
+    const int w = static_cast<int>(blockIdx.x);
+    int at = 0;
+    if (seqs.count > 1) {
+        // Sequences that end at or before unit w: every lane looks at two of them.
+        const int lane = threadIdx.x % kWave;
+        const int e0 = lane < seqs.count ? seqs.seq[lane].unit_end : 0x7fffffff;
+        const int e1 = lane + kWave < seqs.count ? seqs.seq[lane + kWave].unit_end : 0x7fffffff;
+        at = __popcll(__builtin_amdgcn_ballot_w64(e0 <= w)) + __popcll(__builtin_amdgcn_ballot_w64(e1 <= w));
+        at = __builtin_amdgcn_readfirstlane(at);
+    }
+    PagedUnit u;
+    u.seq = seqs.seq[at];
+    const uint32_t local = static_cast<uint32_t>(w - (at > 0 ? seqs.seq[at - 1].unit_end : 0));
+    // KV heads fastest: workgroups are dealt to the XCDs in turn, so with 8 KV heads (or a multiple)
+    // an XCD's L2 sees the keys of one of them. Longest row tiles first.
+    const uint32_t rest = local / static_cast<uint32_t>(kv_heads);
+    u.h_kv = static_cast<int>(local - rest * static_cast<uint32_t>(kv_heads));
+    const uint32_t t = rest / static_cast<uint32_t>(u.seq.splits);
+    u.split = static_cast<int>(rest - t * static_cast<uint32_t>(u.seq.splits));
+    u.tile = u.seq.row_tiles - 1 - static_cast<int>(t);
+    return u;
+}
+
+// Keys that the rows of a tile see at most: all, or up to its last token's own position.
+__device__ __forceinline__ int VisibleKeys(const PagedSeq& s, int tile, int group, bool causal) {
+    if (!causal) return s.keys;
+    const int last_row = min((tile + 1) * kPagedRows, s.q_count * group) - 1;
+    const int last = static_cast<int>(static_cast<uint32_t>(last_row) / static_cast<uint32_t>(group));
+    return max(0, min(s.keys, last + s.keys - s.q_count + 1));
+}
+
+}  // namespace
+}  // namespace sca_hip

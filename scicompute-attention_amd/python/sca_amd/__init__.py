@@ -20,6 +20,9 @@ from .hip import (  # noqa: F401
     FlashParams,
     DecodeParams,
     KvShape,
+    Kv8Layer,
+    Decode8Params,
+    PagedVarlenParams,
     DTYPE_F32,
     DTYPE_F16,
     DTYPE_BF16,

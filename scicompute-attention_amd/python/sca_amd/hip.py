@@ -97,6 +97,28 @@ class KvShape(ctypes.Structure):
                 ("head_dim", c_i64)]
 
 
+class Kv8Layer(ctypes.Structure):
+    """sca_kv8_layer: one layer's 8-bit pages (codes and exponent bytes)."""
+
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_exp", c_vp), ("v_exp", c_vp)]
+
+
+class Decode8Params(ctypes.Structure):
+    _fields_ = [("base", DecodeParams), ("k_exp", c_vp), ("v_exp", c_vp)]
+
+
+class PagedVarlenParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("k", c_vp), ("v", c_vp), ("k_exp", c_vp), ("v_exp", c_vp), ("out", c_vp),
+        ("lse", c_vp), ("page_table", c_vp), ("cu_seqlens_q", c_vp), ("kv_lens", c_vp),
+        ("table_rows", c_vp), ("num_seqs", c_i64), ("num_heads", c_i64), ("num_kv_heads", c_i64),
+        ("head_dim", c_i64), ("block_size", c_i64), ("max_blocks_per_seq", c_i64),
+        ("num_kv_blocks", c_i64), ("q_ss", c_i64), ("q_sh", c_i64), ("k_ss", c_i64), ("k_sh", c_i64),
+        ("v_ss", c_i64), ("v_sh", c_i64), ("o_ss", c_i64), ("o_sh", c_i64), ("scale", ctypes.c_float),
+        ("causal", c_i32), ("dtype", c_i32),
+    ]
+
+
 _LIB = None
 
 
@@ -145,6 +167,16 @@ def hip_lib() -> ctypes.CDLL:
                                             c_i64, c_vp]
     lib.sca_hip_kv_gather.argtypes = [c_vp, c_vp, c_i64, c_vp, ctypes.POINTER(KvShape), c_i64,
                                       c_vp]
+    lib.sca_hip_kv8_append.argtypes = [ctypes.POINTER(Kv8Layer), c_vp, c_vp, c_vp, c_i64,
+                                       ctypes.POINTER(KvShape), c_i32, c_vp]
+    lib.sca_hip_kv8_reset_blocks.argtypes = [ctypes.POINTER(Kv8Layer), c_vp, c_i64,
+                                             ctypes.POINTER(KvShape), c_vp]
+    lib.sca_hip_kv8_gather.argtypes = [c_vp, c_vp, c_vp, c_i64, c_vp, ctypes.POINTER(KvShape), c_i32,
+                                       c_vp]
+    lib.sca_hip_decode8_paged.argtypes = [ctypes.POINTER(Decode8Params), c_vp]
+    lib.sca_hip_paged_varlen_bytes.argtypes = [ctypes.POINTER(PagedVarlenParams)]
+    lib.sca_hip_paged_varlen_bytes.restype = c_i64
+    lib.sca_hip_paged_varlen.argtypes = [ctypes.POINTER(PagedVarlenParams), c_vp, c_i64, c_vp]
     _LIB = lib
     return lib
 
@@ -278,3 +310,16 @@ def decode_splitk_paged(params: DecodeParams, stream=None) -> None:
 def decode_splitk_noalloc(params: DecodeParams, stream=None) -> None:
     """The allocation-free decode entry point: partial_m/l/o and batch_order must be None."""
     check(hip_lib().sca_hip_decode_splitk_noalloc(ctypes.byref(params), stream))
+
+
+def decode8_paged(params: Decode8Params, stream=None) -> None:
+    check(hip_lib().sca_hip_decode8_paged(ctypes.byref(params), stream))
+
+
+def paged_varlen_bytes(params: PagedVarlenParams) -> int:
+    return hip_lib().sca_hip_paged_varlen_bytes(ctypes.byref(params))
+
+
+def paged_varlen(params: PagedVarlenParams, scratch: int | None = None, scratch_bytes: int = 0,
+                 stream=None) -> None:
+    check(hip_lib().sca_hip_paged_varlen(ctypes.byref(params), scratch, scratch_bytes, stream))

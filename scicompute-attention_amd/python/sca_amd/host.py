@@ -21,6 +21,7 @@ c_char_p = ctypes.c_char_p
 
 BACKENDS = {"auto": 0, "naive": 1, "tiled": 2, "flash": 3, "decode": 4, "paged": 5}
 LAYOUTS = {"bhsd": 0, "bshd": 1}
+STORAGES = {"same": 0, "e4m3": 1}
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "i32": 4, "u8": 8}
 ELEM = {"f32": 4, "f16": 2, "bf16": 2, "i32": 4, "u8": 1}
 HOST, GPU = 0, 1
@@ -70,6 +71,11 @@ class ScaPagedParams(ctypes.Structure):
                 ("block_size", c_i64), ("max_blocks_per_seq", c_i64), ("layer", c_i64)]
 
 
+class ScaPagedVarlenParams(ctypes.Structure):
+    _fields_ = [("seq_ids", c_vp), ("kv_lens", c_vp), ("num_seqs", c_i64), ("layer", c_i64),
+                ("page_table", c_vp), ("max_blocks_per_seq", c_i64)]
+
+
 _LIB = None
 
 # (name, restype, argtypes)
@@ -103,6 +109,9 @@ _SIGS = [
     ("sca_compute_slot_mapping", ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp]),
     ("sca_kv_cache_bytes", ctypes.c_int, [ctypes.POINTER(ScaKvConfig), ctypes.POINTER(c_u64)]),
     ("sca_max_blocks_for_budget", c_i64, [ctypes.POINTER(ScaKvConfig), c_u64]),
+    ("sca_kv_cache_bytes_stored", ctypes.c_int, [ctypes.POINTER(ScaKvConfig), c_i32,
+                                                 ctypes.POINTER(c_u64)]),
+    ("sca_max_blocks_for_budget_stored", c_i64, [ctypes.POINTER(ScaKvConfig), c_i32, c_u64]),
     ("sca_tensor_new", c_vp, [ctypes.POINTER(c_i64), c_i32, c_i32, c_i32]),
     ("sca_tensor_wrap", c_vp, [c_vp, ctypes.POINTER(c_i64), c_i32, c_i32, c_i32]),
     ("sca_tensor_free", None, [c_vp]),
@@ -121,6 +130,7 @@ _SIGS = [
     ("sca_explain_tensors", None, [c_vp, c_vp, c_vp, ctypes.POINTER(ScaConfig), c_char_p,
                                    ctypes.c_size_t]),
     ("sca_pkv_create", c_vp, [ctypes.POINTER(ScaKvConfig), c_i32]),
+    ("sca_pkv_create_stored", c_vp, [ctypes.POINTER(ScaKvConfig), c_i32, c_i32]),
     ("sca_pkv_destroy", None, [c_vp]),
     ("sca_pkv_append", ctypes.c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     ("sca_pkv_append_batch", ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
@@ -141,11 +151,16 @@ _SIGS = [
     ("sca_pkv_stats", None, [c_vp, ctypes.POINTER(ScaKvStats)]),
     ("sca_pkv_layer_k", c_vp, [c_vp, c_i64]),
     ("sca_pkv_layer_v", c_vp, [c_vp, c_i64]),
+    ("sca_pkv_layer_k_exponents", c_vp, [c_vp, c_i64]),
+    ("sca_pkv_layer_v_exponents", c_vp, [c_vp, c_i64]),
     ("sca_pkv_blocks", c_vp, [c_vp]),
     ("sca_pkv_gather", ctypes.c_int, [c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, ctypes.POINTER(c_vp)]),
     ("sca_run_paged", ctypes.c_int, [c_vp, c_vp, ctypes.POINTER(ScaPagedParams),
                                      ctypes.POINTER(ScaConfig), ctypes.POINTER(c_vp),
                                      ctypes.POINTER(ScaStats)]),
+    ("sca_run_paged_varlen", ctypes.c_int, [c_vp, c_vp, ctypes.POINTER(ScaPagedVarlenParams),
+                                            ctypes.POINTER(ScaConfig), ctypes.POINTER(c_vp),
+                                            ctypes.POINTER(c_vp), ctypes.POINTER(ScaStats)]),
     ("sca_bm_create", c_vp, [c_i64, c_i64, c_i64, c_i32]),
     ("sca_bm_destroy", None, [c_vp]),
     ("sca_bm_allocate", ctypes.c_int, [c_vp, c_i64, c_vp]),
@@ -267,6 +282,11 @@ class KVCacheConfig:
     max_num_seqs: int = 1
     dtype: str = "f16"
     layout: int = 0
+    storage: str | int = "same"  # "e4m3": 8-bit codes with exponent bytes, standing for dtype
+
+    @property
+    def storage_id(self) -> int:
+        return STORAGES[self.storage] if isinstance(self.storage, str) else int(self.storage)
 
     def to_c(self) -> ScaKvConfig:
         return ScaKvConfig(self.num_layers, self.num_kv_heads, self.head_dim, self.block_size,
@@ -474,13 +494,13 @@ def compute_slot_mapping(row, seq_start, num_tokens, block_size, max_blocks):
 def kv_cache_bytes(cfg: KVCacheConfig) -> int:
     c = cfg.to_c()
     out = c_u64()
-    _raise(host_lib().sca_kv_cache_bytes(ctypes.byref(c), ctypes.byref(out)))
+    _raise(host_lib().sca_kv_cache_bytes_stored(ctypes.byref(c), cfg.storage_id, ctypes.byref(out)))
     return out.value
 
 
 def max_blocks_for_budget(cfg: KVCacheConfig, budget: int) -> int:
     c = cfg.to_c()
-    return host_lib().sca_max_blocks_for_budget(ctypes.byref(c), budget)
+    return host_lib().sca_max_blocks_for_budget_stored(ctypes.byref(c), cfg.storage_id, budget)
 
 
 # ---- BlockManager / PagedKVCache / Workspace ------------------------------------------------------
@@ -547,7 +567,7 @@ class PagedKVCache:
         lib = host_lib()
         self.cfg = cfg
         c = cfg.to_c()
-        self.h = lib.sca_pkv_create(ctypes.byref(c), device)
+        self.h = lib.sca_pkv_create_stored(ctypes.byref(c), cfg.storage_id, device)
         if not self.h:
             msg = lib.sca_last_error()
             raise ScaError(lib.sca_extract_code(msg), msg.decode())
@@ -628,6 +648,11 @@ class PagedKVCache:
         lib = host_lib()
         return lib.sca_pkv_layer_k(self.h, layer), lib.sca_pkv_layer_v(self.h, layer)
 
+    def layer_exponent_ptrs(self, layer=0):
+        """Exponent bytes of K and V with 8-bit storage, [num_blocks, num_kv_heads, block_size]."""
+        lib = host_lib()
+        return lib.sca_pkv_layer_k_exponents(self.h, layer), lib.sca_pkv_layer_v_exponents(self.h, layer)
+
     def blocks(self) -> BlockManager:
         return BlockManager(0, self.cfg.max_num_seqs, self.max_blocks_per_seq,
                             _borrowed=host_lib().sca_pkv_blocks(self.h))
@@ -661,6 +686,36 @@ def paged_attention(q: Tensor, kv: PagedKVCache, params: dict | None = None, cfg
     _raise(host_lib().sca_run_paged(q.handle, kv.h, p_ptr, ctypes.byref(c), ctypes.byref(out),
                                     ctypes.byref(st)))
     return AttentionResult(Tensor(out.value, q.dtype), None, _stats(st))
+
+
+def paged_attention_varlen(q: Tensor, kv: PagedKVCache, params: dict, cfg: AttentionConfig):
+    """Ragged chunks of new tokens (packed q [T, H_q, D], cfg.cu_seqlens_q) over a paged cache that
+    holds them already. params: num_seqs, and optionally layer, seq_ids (the cache's sequences),
+    kv_lens (keys to attend), page_table (device) with max_blocks_per_seq."""
+    c = cfg.to_c()
+    n = int(params.get("num_seqs", 0))
+    keep = []
+
+    def array(name, dtype):
+        a = params.get(name)
+        if a is None:
+            return None
+        a = np.ascontiguousarray(a, dtype=dtype)
+        if a.size != n:
+            raise ValueError(f"{name} has {a.size} entries for {n} sequences")
+        keep.append(a)
+        return a.ctypes.data
+
+    if cfg.cu_seqlens_q is not None and np.size(cfg.cu_seqlens_q) != n + 1:
+        raise ValueError(f"cu_seqlens_q has {np.size(cfg.cu_seqlens_q)} entries for {n} sequences")
+    p = ScaPagedVarlenParams(array("seq_ids", np.int64), array("kv_lens", np.int32), n,
+                             params.get("layer", 0), params.get("page_table"),
+                             params.get("max_blocks_per_seq", 0))
+    out, lse, st = c_vp(), c_vp(), ScaStats()
+    _raise(host_lib().sca_run_paged_varlen(q.handle, kv.h, ctypes.byref(p), ctypes.byref(c),
+                                           ctypes.byref(out), ctypes.byref(lse), ctypes.byref(st)))
+    lse_t = Tensor(lse.value, "f32") if lse.value else None
+    return AttentionResult(Tensor(out.value, q.dtype), lse_t, _stats(st))
 
 
 class Workspace:

@@ -78,6 +78,14 @@ const char* LayoutName(AttnLayout layout) noexcept {
     return "unknown-layout";
 }
 
+const char* KvStorageName(KvStorage storage) noexcept {
+    switch (storage) {
+        case KvStorage::kSame: return "same";
+        case KvStorage::kE4M3: return "e4m3";
+    }
+    return "unknown";
+}
+
 const char* KvLayoutName(KvLayout layout) noexcept {
     return layout == KvLayout::kBlockMajor ? "block-major" : "unknown-kv-layout";
 }

@@ -323,6 +323,13 @@ sci::Result<AttentionResult> RunPaged(const sci::Tensor& q, const PagedKVCache& 
                     "paged_attention has no page table (call PagedKVCache::SyncPageTable first)");
     }
     const int64_t block_size = params.block_size > 0 ? params.block_size : kv.BlockSize();
+    const bool held8 = kv_cfg.storage == KvStorage::kE4M3;
+    if (held8 && block_size != kv.BlockSize()) {
+        // The exponent bytes are laid out by the cache's own pages.
+        return fail(AttnStatusCode::kShapeMismatch,
+                    "paged_attention block_size=" + std::to_string(block_size) +
+                        " differs from the 8-bit cache's " + std::to_string(kv.BlockSize()));
+    }
     const int64_t max_blocks =
         params.max_blocks_per_seq > 0 ? params.max_blocks_per_seq : kv.MaxBlocksPerSeq();
     // Upper bound of a sequence's length; the kernel reads the true lengths from seq_lens.
@@ -343,7 +350,14 @@ sci::Result<AttentionResult> RunPaged(const sci::Tensor& q, const PagedKVCache& 
         const int cus = DeviceCapability::ForDevice(0).sm_count;
         std::vector<int64_t> lengths(static_cast<size_t>(num_seqs));
         for (int64_t b = 0; b < num_seqs; ++b) lengths[static_cast<size_t>(b)] = kv.SeqLength(b);
-        if (detail::PagedValuGroup(head_dim, num_heads / kv_cfg.num_kv_heads)) {
+        if (held8) {
+            const auto plan = detail::PagedDecode8PlanFor(head_dim, lengths.data(), num_seqs, num_heads,
+                                                          kv_cfg.num_kv_heads, cus);
+            if (plan.slot_waves != 0) {
+                splits = plan.splits;
+                slot_waves = plan.slot_waves;
+            }
+        } else if (detail::PagedValuGroup(head_dim, num_heads / kv_cfg.num_kv_heads)) {
             splits = detail::PagedValuSplits(head_dim, lengths.data(), num_seqs, num_heads,
                                              kv_cfg.num_kv_heads, cus);
         } else {
@@ -389,7 +403,14 @@ sci::Result<AttentionResult> RunPaged(const sci::Tensor& q, const PagedKVCache& 
     p.slot_waves = slot_waves;
     size_t partial_bytes = 0;
     sci::Status status = BindPartials(&p, splits, q.device().id(), &partial_bytes);
-    if (status.ok()) {
+    if (status.ok() && held8) {
+        sca_decode8_params p8{};
+        p8.base = p;
+        p8.k_exp = static_cast<const uint8_t*>(kv.Storage().KExponents(params.layer).data());
+        p8.v_exp = static_cast<const uint8_t*>(kv.Storage().VExponents(params.layer).data());
+        status = runtime::StatusFromHip(sca_hip_decode8_paged(&p8, runtime::StreamHandle(cfg.stream)),
+                                        "paged decode (8-bit pages)");
+    } else if (status.ok()) {
         status = runtime::StatusFromHip(
             sca_hip_decode_splitk_paged(&p, runtime::StreamHandle(cfg.stream)), "paged decode");
     }
@@ -400,7 +421,8 @@ sci::Result<AttentionResult> RunPaged(const sci::Tensor& q, const PagedKVCache& 
     result.stats.kv_bytes = kv.Storage().MemoryBytes();
     result.stats.note = "paged decode: " + std::to_string(splits) + " splits, " +
                         (slot_waves == 4 ? "four waves" : "one wave") + " per head slot, block_size=" +
-                        std::to_string(block_size) + ", layer=" + std::to_string(params.layer);
+                        std::to_string(block_size) + ", layer=" + std::to_string(params.layer) +
+                        (held8 ? ", 8-bit pages" : "");
     return sci::Ok(std::move(result));
 }
 

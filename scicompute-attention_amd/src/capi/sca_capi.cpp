@@ -5,6 +5,7 @@
 #include "sca_capi.h"
 
 #include <cstring>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -77,7 +78,7 @@ sca::AttentionShape ToShape(const ScaShape* s) {
     return shape;
 }
 
-sca::KVCacheConfig ToKvCfg(const ScaKvConfig* c) {
+sca::KVCacheConfig ToKvCfg(const ScaKvConfig* c, int32_t storage = 0) {
     sca::KVCacheConfig cfg;
     cfg.num_layers = c->num_layers;
     cfg.num_kv_heads = c->num_kv_heads;
@@ -87,6 +88,7 @@ sca::KVCacheConfig ToKvCfg(const ScaKvConfig* c) {
     cfg.max_num_seqs = c->max_num_seqs;
     cfg.dtype = static_cast<sci::DType>(c->dtype);
     cfg.layout = static_cast<sca::KvLayout>(c->layout);
+    cfg.storage = static_cast<sca::KvStorage>(storage);
     return cfg;
 }
 
@@ -259,6 +261,15 @@ int sca_kv_cache_bytes(const ScaKvConfig* cfg, uint64_t* bytes) {
 int64_t sca_max_blocks_for_budget(const ScaKvConfig* cfg, uint64_t budget_bytes) {
     return sca::MaxBlocksForBudget(ToKvCfg(cfg), budget_bytes);
 }
+int sca_kv_cache_bytes_stored(const ScaKvConfig* cfg, int32_t storage, uint64_t* bytes) {
+    const auto r = sca::KvCacheBytes(ToKvCfg(cfg, storage));
+    if (!r.ok()) return Fail(r.error());
+    if (bytes != nullptr) *bytes = *r;
+    return 0;
+}
+int64_t sca_max_blocks_for_budget_stored(const ScaKvConfig* cfg, int32_t storage, uint64_t budget_bytes) {
+    return sca::MaxBlocksForBudget(ToKvCfg(cfg, storage), budget_bytes);
+}
 
 // ---- tensors ----
 ScaTensor* sca_tensor_new(const int64_t* dims, int32_t ndims, int32_t dtype, int32_t device_kind) {
@@ -330,6 +341,14 @@ void sca_explain_tensors(const ScaTensor* q, const ScaTensor* k, const ScaTensor
 // ---- paged KV cache ----
 ScaPagedKV* sca_pkv_create(const ScaKvConfig* cfg, int32_t device_kind) {
     auto r = sca::PagedKVCache::Create(ToKvCfg(cfg), DeviceOf(device_kind));
+    if (!r.ok()) {
+        Fail(r.error());
+        return nullptr;
+    }
+    return reinterpret_cast<ScaPagedKV*>(new sca::PagedKVCache(std::move(*r)));
+}
+ScaPagedKV* sca_pkv_create_stored(const ScaKvConfig* cfg, int32_t storage, int32_t device_kind) {
+    auto r = sca::PagedKVCache::Create(ToKvCfg(cfg, storage), DeviceOf(device_kind));
     if (!r.ok()) {
         Fail(r.error());
         return nullptr;
@@ -410,6 +429,12 @@ void* sca_pkv_layer_k(const ScaPagedKV* c, int64_t layer) {
 void* sca_pkv_layer_v(const ScaPagedKV* c, int64_t layer) {
     return const_cast<void*>(P(c).Storage().V(layer).data());
 }
+void* sca_pkv_layer_k_exponents(const ScaPagedKV* c, int64_t layer) {
+    return const_cast<void*>(P(c).Storage().KExponents(layer).data());
+}
+void* sca_pkv_layer_v_exponents(const ScaPagedKV* c, int64_t layer) {
+    return const_cast<void*>(P(c).Storage().VExponents(layer).data());
+}
 const ScaBlockManager* sca_pkv_blocks(const ScaPagedKV* c) {
     return reinterpret_cast<const ScaBlockManager*>(&P(c).Blocks());
 }
@@ -438,6 +463,27 @@ int sca_run_paged(const ScaTensor* q, const ScaPagedKV* kv, const ScaPagedParams
     p.max_blocks_per_seq = params->max_blocks_per_seq;
     p.layer = params->layer;
     return Finish(sca::paged_attention(T(q), P(kv), p, h.cfg), false, out, nullptr, stats);
+}
+
+int sca_run_paged_varlen(const ScaTensor* q, const ScaPagedKV* kv, const ScaPagedVarlenParams* params,
+                         const ScaConfig* cfg, ScaTensor** out, ScaTensor** lse, ScaStats* stats) {
+    if (q == nullptr || kv == nullptr || params == nullptr || cfg == nullptr) {
+        return Fail(sca::MakeStatus(sca::AttnStatusCode::kShapeMismatch, "sca_run_paged_varlen: null pointer"));
+    }
+    try {  // (the lengths of a call are copied into host memory)
+        CfgHolder h;
+        ToCfg(cfg, &h);
+        sca::PagedVarlenParams p;
+        p.seq_ids = params->seq_ids;
+        p.kv_lens = params->kv_lens;
+        p.num_seqs = params->num_seqs;
+        p.layer = params->layer;
+        p.page_table = params->page_table;
+        p.max_blocks_per_seq = params->max_blocks_per_seq;
+        return Finish(sca::paged_attention_varlen(T(q), P(kv), p, h.cfg), h.cfg.return_lse, out, lse, stats);
+    } catch (const std::exception& e) {
+        return Fail(sca::MakeStatus(sca::AttnStatusCode::kWorkspaceExceeded, e.what()));
+    }
 }
 
 // ---- BlockManager ----

@@ -20,6 +20,13 @@ bool SupportedBlockSize(int64_t bs) {
     return bs == 1 || bs == 8 || bs == 16 || bs == 32 || bs == 64;
 }
 
+bool Held8(const KVCacheConfig& cfg) { return cfg.storage == KvStorage::kE4M3; }
+
+// Bytes of one token's K (or V) of one head.
+int64_t RowBytes(const KVCacheConfig& cfg) {
+    return Held8(cfg) ? cfg.head_dim + 1 : cfg.head_dim * DtypeSize(cfg.dtype);
+}
+
 sci::Status CheckConfig(const KVCacheConfig& cfg) {
     auto bad = [](AttnStatusCode code, const std::string& what) {
         return MakeStatus(code, "KVCacheConfig invalid: " + what);
@@ -54,6 +61,17 @@ sci::Status CheckConfig(const KVCacheConfig& cfg) {
                    std::string("layout=") + KvLayoutName(cfg.layout) +
                        " (v1 implements block-major only)");
     }
+    if (cfg.storage != KvStorage::kSame && cfg.storage != KvStorage::kE4M3) {
+        return bad(AttnStatusCode::kUnsupportedFeature,
+                   "storage=" + std::to_string(static_cast<int>(cfg.storage)));
+    }
+    if (Held8(cfg) && cfg.dtype == sci::DType::kFloat32) {
+        return bad(AttnStatusCode::kUnsupportedDtype, "8-bit storage stands for float16 or bfloat16; dtype=float32");
+    }
+    if (Held8(cfg) && cfg.block_size < 8) {
+        return bad(AttnStatusCode::kShapeMismatch, "block_size=" + std::to_string(cfg.block_size) +
+                                                       " (8-bit storage: 8, 16, 32, 64)");
+    }
     return sci::Status::Ok();
 }
 
@@ -66,6 +84,15 @@ sca_kv_shape KernelShape(const KVCacheConfig& cfg) {
     return s;
 }
 
+sca_kv8_layer Layer8(sci::Tensor& k, sci::Tensor& v, sci::Tensor& k_exp, sci::Tensor& v_exp) {
+    sca_kv8_layer l{};
+    l.k = k.data();
+    l.v = v.data();
+    l.k_exp = static_cast<uint8_t*>(k_exp.data());
+    l.v_exp = static_cast<uint8_t*>(v_exp.data());
+    return l;
+}
+
 std::string Mib(size_t bytes) { return std::to_string(bytes / (1024 * 1024)); }
 
 }  // namespace
@@ -73,8 +100,8 @@ std::string Mib(size_t bytes) { return std::to_string(bytes / (1024 * 1024)); }
 sci::Result<size_t> KvCacheBytes(const KVCacheConfig& cfg) {
     const sci::Status valid = CheckConfig(cfg);
     if (!valid.ok()) return sci::MakeUnexpected<size_t>(valid);
-    const int64_t per_layer = cfg.num_blocks * cfg.block_size * cfg.num_kv_heads * cfg.head_dim;
-    const int64_t total = 2 * cfg.num_layers * per_layer * DtypeSize(cfg.dtype);
+    const int64_t per_layer = cfg.num_blocks * cfg.block_size * cfg.num_kv_heads * RowBytes(cfg);
+    const int64_t total = 2 * cfg.num_layers * per_layer;
     if (total <= 0) {
         return sci::MakeUnexpected<size_t>(
             MakeStatus(AttnStatusCode::kShapeMismatch, "KVCacheConfig overflow"));
@@ -83,8 +110,8 @@ sci::Result<size_t> KvCacheBytes(const KVCacheConfig& cfg) {
 }
 
 int64_t MaxBlocksForBudget(const KVCacheConfig& cfg, size_t budget_bytes) {
-    const int64_t per_block = 2 * cfg.num_layers * cfg.block_size * cfg.num_kv_heads *
-                              cfg.head_dim * DtypeSize(cfg.dtype);
+    const int64_t per_block =
+        2 * cfg.num_layers * cfg.block_size * cfg.num_kv_heads * RowBytes(cfg);
     if (per_block <= 0) return 0;
     return static_cast<int64_t>(budget_bytes / static_cast<size_t>(per_block));
 }
@@ -151,12 +178,23 @@ sci::Result<KVCache> KVCache::Create(const KVCacheConfig& cfg, sci::Device& devi
                                         cfg.head_dim});
     cache.k_layers_.reserve(static_cast<size_t>(cfg.num_layers));
     cache.v_layers_.reserve(static_cast<size_t>(cfg.num_layers));
-    const size_t layer_bytes = static_cast<size_t>(cache.layer_elements_) *
-                               static_cast<size_t>(DtypeSize(cfg.dtype));
+    const sci::DType kept = Held8(cfg) ? sci::DType::kUInt8 : cfg.dtype;
+    const size_t layer_bytes =
+        static_cast<size_t>(cache.layer_elements_) * static_cast<size_t>(sci::kDTypeSize(kept));
+    const sci::TensorShape exponent_shape({cfg.num_blocks, cfg.num_kv_heads, cfg.block_size});
+    const size_t exponent_bytes =
+        static_cast<size_t>(cfg.num_blocks * cfg.num_kv_heads * cfg.block_size);
     for (int64_t layer = 0; layer < cfg.num_layers; ++layer) {
-        cache.k_layers_.emplace_back(layer_shape, cfg.dtype, device);
-        cache.v_layers_.emplace_back(layer_shape, cfg.dtype, device);
-        if (cache.k_layers_.back().data() == nullptr || cache.v_layers_.back().data() == nullptr) {
+        cache.k_layers_.emplace_back(layer_shape, kept, device);
+        cache.v_layers_.emplace_back(layer_shape, kept, device);
+        bool got = cache.k_layers_.back().data() != nullptr && cache.v_layers_.back().data() != nullptr;
+        if (Held8(cfg)) {
+            cache.k_exponents_.emplace_back(exponent_shape, sci::DType::kUInt8, device);
+            cache.v_exponents_.emplace_back(exponent_shape, sci::DType::kUInt8, device);
+            got = got && cache.k_exponents_.back().data() != nullptr &&
+                  cache.v_exponents_.back().data() != nullptr;
+        }
+        if (!got) {
             return sci::MakeUnexpected<KVCache>(MakeStatus(
                 AttnStatusCode::kKVCapacityExceeded,
                 "KV cache allocation failed at layer " + std::to_string(layer) + " (" +
@@ -165,6 +203,10 @@ sci::Result<KVCache> KVCache::Create(const KVCacheConfig& cfg, sci::Device& devi
         // Pages start zeroed, as after a Reset().
         device.memset(cache.k_layers_.back().data(), 0, layer_bytes);
         device.memset(cache.v_layers_.back().data(), 0, layer_bytes);
+        if (Held8(cfg)) {
+            device.memset(cache.k_exponents_.back().data(), 0, exponent_bytes);
+            device.memset(cache.v_exponents_.back().data(), 0, exponent_bytes);
+        }
     }
     cache.stats_.num_blocks = cfg.num_blocks;
     cache.stats_.free_blocks = cfg.num_blocks;
@@ -200,11 +242,17 @@ sci::Status KVCache::Append(int64_t layer, const sci::Tensor& k_new, const sci::
     }
     const sca_kv_shape shape = KernelShape(cfg_);
     const size_t l = static_cast<size_t>(layer);
-    const sci::Status status = runtime::StatusFromHip(
-        sca_hip_kv_append(k_layers_[l].data(), v_layers_[l].data(), k_new.data(), v_new.data(),
-                          slot_mapping, num_tokens, &shape, DtypeSize(cfg_.dtype),
-                          runtime::StreamHandle(stream)),
-        "KVCache::Append");
+    int rc = 0;
+    if (Held8(cfg_)) {
+        const sca_kv8_layer held = Layer8(k_layers_[l], v_layers_[l], k_exponents_[l], v_exponents_[l]);
+        rc = sca_hip_kv8_append(&held, k_new.data(), v_new.data(), slot_mapping, num_tokens, &shape,
+                                runtime::KernelDtype(cfg_.dtype), runtime::StreamHandle(stream));
+    } else {
+        rc = sca_hip_kv_append(k_layers_[l].data(), v_layers_[l].data(), k_new.data(), v_new.data(),
+                               slot_mapping, num_tokens, &shape, DtypeSize(cfg_.dtype),
+                               runtime::StreamHandle(stream));
+    }
+    const sci::Status status = runtime::StatusFromHip(rc, "KVCache::Append");
     if (!status.ok()) return status;
     ++stats_.num_appends;
     return sci::Status::Ok();
@@ -242,10 +290,18 @@ sci::Result<sci::Tensor> KVCache::GatherInternal(int64_t layer, const int32_t* b
             MakeStatus(AttnStatusCode::kWorkspaceExceeded, "KVCache::Gather allocation failed"));
     }
     const sca_kv_shape shape = KernelShape(cfg_);
-    const sci::Status status = runtime::StatusFromHip(
-        sca_hip_kv_gather(src.data(), block_ids, num_blocks, out.data(), &shape,
-                          DtypeSize(cfg_.dtype), runtime::StreamHandle(stream)),
-        "KVCache::Gather");
+    int rc = 0;
+    if (Held8(cfg_)) {
+        const sci::Tensor& e = is_key ? k_exponents_[static_cast<size_t>(layer)]
+                                      : v_exponents_[static_cast<size_t>(layer)];
+        rc = sca_hip_kv8_gather(src.data(), static_cast<const uint8_t*>(e.data()), block_ids, num_blocks,
+                                out.data(), &shape, runtime::KernelDtype(cfg_.dtype),
+                                runtime::StreamHandle(stream));
+    } else {
+        rc = sca_hip_kv_gather(src.data(), block_ids, num_blocks, out.data(), &shape,
+                               DtypeSize(cfg_.dtype), runtime::StreamHandle(stream));
+    }
+    const sci::Status status = runtime::StatusFromHip(rc, "KVCache::Gather");
     if (!status.ok()) return sci::MakeUnexpected<sci::Tensor>(status);
     return sci::Ok(std::move(out));
 }
@@ -258,15 +314,35 @@ sci::Status KVCache::Reset(const int32_t* block_ids, int64_t num_blocks, sci::St
     const sca_kv_shape shape = KernelShape(cfg_);
     for (int64_t layer = 0; layer < cfg_.num_layers; ++layer) {
         const size_t l = static_cast<size_t>(layer);
-        const sci::Status status = runtime::StatusFromHip(
-            sca_hip_kv_reset_blocks(k_layers_[l].data(), v_layers_[l].data(), block_ids,
-                                    num_blocks, &shape, DtypeSize(cfg_.dtype),
-                                    runtime::StreamHandle(stream)),
-            "KVCache::Reset");
+        int rc = 0;
+        if (Held8(cfg_)) {
+            const sca_kv8_layer held = Layer8(k_layers_[l], v_layers_[l], k_exponents_[l], v_exponents_[l]);
+            rc = sca_hip_kv8_reset_blocks(&held, block_ids, num_blocks, &shape,
+                                          runtime::StreamHandle(stream));
+        } else {
+            rc = sca_hip_kv_reset_blocks(k_layers_[l].data(), v_layers_[l].data(), block_ids,
+                                         num_blocks, &shape, DtypeSize(cfg_.dtype),
+                                         runtime::StreamHandle(stream));
+        }
+        const sci::Status status = runtime::StatusFromHip(rc, "KVCache::Reset");
         if (!status.ok()) return status;
     }
     ++stats_.num_resets;
     return sci::Status::Ok();
+}
+
+const sci::Tensor& KVCache::KExponents(int64_t layer) const {
+    static const sci::Tensor kNone;
+    return layer >= 0 && layer < static_cast<int64_t>(k_exponents_.size())
+               ? k_exponents_[static_cast<size_t>(layer)]
+               : kNone;
+}
+
+const sci::Tensor& KVCache::VExponents(int64_t layer) const {
+    static const sci::Tensor kNone;
+    return layer >= 0 && layer < static_cast<int64_t>(v_exponents_.size())
+               ? v_exponents_[static_cast<size_t>(layer)]
+               : kNone;
 }
 
 const sci::Tensor& KVCache::K(int64_t layer) const {

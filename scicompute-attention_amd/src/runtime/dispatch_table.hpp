@@ -253,5 +253,12 @@ inline PagedDecodePlanResult PagedDecodePlanFor(int64_t head_dim, const int64_t*
     return plan;
 }
 
+// The same over 8-bit pages.
+inline PagedDecodePlanResult PagedDecode8PlanFor(int64_t head_dim, const int64_t* lengths, int64_t batch,
+                                                 int64_t num_heads, int64_t num_kv_heads,
+                                                 int64_t cu_count) {
+    return PagedDecodePlanFor(head_dim, lengths, batch, num_heads, num_kv_heads, cu_count);
+}
+
 }  // namespace detail
 }  // namespace sca
