@@ -15,7 +15,6 @@
 //     (in fp16 a weight times a small 2^k would leave the type's range).
 //   * Exponents: one byte load per lane and tile (lanes 0-31 the tokens of K, 32-63 of V), handed to
 //     the lanes that need them with shuffles.
-// Both tiles of a wave in flight are in registers (2 x (K + V) x D/8 registers at most).
 
 #include <hip/hip_runtime.h>
 
@@ -28,6 +27,9 @@
 namespace sca_hip {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 template <int D>
 struct Dec8Geom {
     static constexpr int N16 = D / 64;            // 16-byte K loads per lane and row
@@ -38,27 +40,17 @@ struct Dec8Geom {
     static constexpr int CPR = D / 16;            // 16-code chunks per row
     static constexpr int NV = kMfmaTile * CPR / kWave;  // V loads per lane and tile
     static constexpr int TILE_BYTES = kMfmaTile * RB;
+    // Waves per SIMD that the registers are kept to (O, Q and a tile's codes); more than one also keeps
+    // O in the ordinary registers, where its rescaling needs no copies.
+    static constexpr int WAVES = D <= 32 ? 6 : D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? 3 : 2;
     static_assert(NV * kWave == kMfmaTile * CPR, "V chunks divide evenly");
     static_assert(kDecodeWaves * kMfmaHeads * D * 4 <= kDecodeWaves * TILE_BYTES, "merge fits the tiles");
 };
 
-// One tile's codes on their way: K rows col and 16 + col of the tile, V chunks, the exponent byte of
-// token lane % 32 (K for the lower half of the wave, V for the upper), and which tokens exist.
-template <int D>
-struct Dec8Tile {
-    using G = Dec8Geom<D>;
-    uint4 k16[2][G::N16 > 0 ? G::N16 : 1];
-    uint2 k8[2];
-    uint4 v[G::NV];
-    uint32_t exponent;
-    uint32_t valid;
-};
-
 template <typename E, int D, bool kWaveHeads>
-__global__ __launch_bounds__(kDecodeThreads) void decode8_kernel(const sca_decode_params p,
-                                                                 const uint8_t* __restrict__ k_exp,
-                                                                 const uint8_t* __restrict__ v_exp,
-                                                                 int h_chunks, int block_shift) {
+__global__ __launch_bounds__(kDecodeThreads, Dec8Geom<D>::WAVES) void decode8_kernel(
+    const sca_decode_params p, const uint8_t* __restrict__ k_exp, const uint8_t* __restrict__ v_exp,
+    int h_chunks, int block_shift) {
     using G = Dec8Geom<D>;
     using T = typename E::Type;
     using M = DecMfma<typename E::Dec>;
@@ -85,7 +77,7 @@ __global__ __launch_bounds__(kDecodeThreads) void decode8_kernel(const sca_decod
     const int64_t h_chunk = slot % static_cast<uint32_t>(h_chunks);
     // The sequence of this workgroup: the blockIdx.z-th longest, as in the 16-bit kernel.
     int64_t b = blockIdx.z;
-    int64_t len = p.seq_kv;
+    int len = static_cast<int>(p.seq_kv);  // (below 2^31, as every token index here)
     if (p.seq_lens != nullptr && p.batch <= kRankBatch) {
         const int tid = threadIdx.x;
         const int nb = static_cast<int>(p.batch);
@@ -139,18 +131,23 @@ __global__ __launch_bounds__(kDecodeThreads) void decode8_kernel(const sca_decod
     float m = neg_inf();  // running max of head `col` (log2 units, identical across lane groups)
     float l = 0.0f;       // this lane's share of the running denominator
 
-    const int64_t chunk = SplitChunk(len, p.num_splits);
-    const int64_t t_begin = split * chunk;
-    const int64_t t_end = (t_begin + chunk < len) ? (t_begin + chunk) : len;
+    const int chunk = static_cast<int>(SplitChunk(len, p.num_splits));
+    const int t_begin = static_cast<int>(min(static_cast<int64_t>(len), split * chunk));
+    const int t_end = len - t_begin < chunk ? len : t_begin + chunk;
     const int n_tiles =
-        slot_ok && t_end > t_begin ? static_cast<int>((t_end - t_begin + kMfmaTile - 1) / kMfmaTile) : 0;
+        slot_ok && t_end > t_begin ? static_cast<int>((static_cast<uint32_t>(t_end - t_begin) + kMfmaTile - 1) / kMfmaTile)
+                                   : 0;
     constexpr int TS = kWaveHeads ? 1 : kDecodeWaves;  // tile stride of one wave
 
     const uint8_t* k_base = static_cast<const uint8_t*>(p.k) + h_kv * p.k_sh;
     const uint8_t* v_base = static_cast<const uint8_t*>(p.v) + h_kv * p.v_sh;
     const uint8_t* exp_base = lane < 32 ? k_exp : v_exp;
     const int32_t* table = p.page_table + b * p.max_blocks_per_seq;
-    const int64_t bs_mask = (int64_t{1} << block_shift) - 1;
+    const uint32_t bs_mask = (1u << block_shift) - 1;
+    // Pool rows and row strides are below 2^31 (checked): one 32 x 32 -> 64 bit product per address.
+    const uint32_t k_row = static_cast<uint32_t>(p.k_ss), v_row = static_cast<uint32_t>(p.v_ss);
+    const uint32_t max_blocks = static_cast<uint32_t>(min(p.max_blocks_per_seq, int64_t{0x7fffffff}));
+    const uint32_t num_blocks = static_cast<uint32_t>(p.num_kv_blocks);
 
     uint8_t* vs = s_v + wave * G::TILE_BYTES;
     const int tr_row = 4 * grp + col / 4;
@@ -159,77 +156,94 @@ __global__ __launch_bounds__(kDecodeThreads) void decode8_kernel(const sca_decod
 
     // Row of token lane % 32 of a tile (< 0: it contributes nothing). Fetched a tile ahead of the
     // tile's loads, which need it.
-    auto row_of = [&](int tile) -> int64_t {
-        const int64_t tok = t_begin + static_cast<int64_t>(tile) * kMfmaTile + lane % 32;
-        const int64_t logical = tok >> block_shift;
-        if (tok >= t_end || logical >= p.max_blocks_per_seq) return -1;
-        const int32_t id = table[logical];
-        if (id < 0 || id >= p.num_kv_blocks) return -1;
-        return (static_cast<int64_t>(id) << block_shift) | (tok & bs_mask);
+    auto row_of = [&](int tile) -> int {
+        const uint32_t tok = static_cast<uint32_t>(t_begin) + static_cast<uint32_t>(tile) * kMfmaTile + lane % 32;
+        const uint32_t logical = tok >> block_shift;
+        if (tok >= static_cast<uint32_t>(t_end) || logical >= max_blocks) return -1;
+        const uint32_t id = static_cast<uint32_t>(table[logical]);  // (negative ids are large ones)
+        return id < num_blocks ? static_cast<int>((id << block_shift) | (tok & bs_mask)) : -1;
     };
-    auto issue = [&](int64_t row, Dec8Tile<D>& t) __attribute__((always_inline)) {
-        t.valid = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(row >= 0));
-        const int safe = row < 0 ? 0 : static_cast<int>(row);  // rows that count for nothing read row 0
-        const int64_t page = safe >> block_shift;
-        t.exponent = exp_base[((page * p.num_kv_heads + h_kv) << block_shift) + (safe & bs_mask)];
+    // A tile's codes on their way, in registers: V is widened into LDS first, and the next tile's V
+    // requested into the same registers at once; K likewise behind the QK products. (Two sets of
+    // registers halve the waves that fit: measured slower.)
+    u32x4 k16[2][G::N16 > 0 ? G::N16 : 1];
+    u32x2 k8[2];
+    u32x4 v[G::NV];
+    uint32_t next_exponent = 0;  // of token lane % 32: K's in the lower half of the wave, V's in the upper
+    uint32_t next_valid = 0;     // tokens that exist
+    uint32_t k_safe[2];          // rows of this lane's two K rows
+    auto issue_v = [&](int row) __attribute__((always_inline)) {
+        next_valid = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(row >= 0)));
+        const uint32_t safe = row < 0 ? 0 : static_cast<uint32_t>(row);  // rows that count for nothing read row 0
+        const uint64_t page_head = static_cast<uint64_t>(safe >> block_shift) * static_cast<uint32_t>(p.num_kv_heads) +
+                                   static_cast<uint32_t>(h_kv);
+        next_exponent = exp_base[(page_head << block_shift) + (safe & bs_mask)];
 #pragma unroll
         for (int i = 0; i < G::NV; ++i) {
             const int c = i * kWave + lane;
-            const int64_t r = __shfl(safe, c / G::CPR);
-            t.v[i] = *reinterpret_cast<const uint4*>(v_base + r * p.v_ss + (c % G::CPR) * 16);
+            const uint32_t r = __shfl(safe, c / G::CPR);
+            v[i] = *reinterpret_cast<const u32x4*>(v_base + static_cast<uint64_t>(r) * v_row + (c % G::CPR) * 16);
         }
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) k_safe[rt] = __shfl(safe, 16 * rt + col);
+    };
+    auto issue_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const int64_t r = __shfl(safe, 16 * rt + col);
-            const uint8_t* src = k_base + r * p.k_ss;
+            const uint8_t* src = k_base + static_cast<uint64_t>(k_safe[rt]) * k_row;
 #pragma unroll
             for (int j = 0; j < G::N16; ++j) {
-                t.k16[rt][j] = *reinterpret_cast<const uint4*>(src + 64 * j + 16 * grp);
+                k16[rt][j] = *reinterpret_cast<const u32x4*>(src + 64 * j + 16 * grp);
             }
-            if constexpr (G::N8) t.k8[rt] = *reinterpret_cast<const uint2*>(src + 64 * G::N16 + 8 * grp);
+            if constexpr (G::N8) k8[rt] = *reinterpret_cast<const u32x2*>(src + 64 * G::N16 + 8 * grp);
         }
     };
-    auto compute = [&](const Dec8Tile<D>& t) __attribute__((always_inline)) {
-        // V into LDS first: its writes run under the QK products.
+    // Tile t; `next_row`: the following tile's rows (`more`: there is one).
+    auto compute = [&](bool more, int next_row) __attribute__((always_inline)) {
+        const uint32_t valid = next_valid, exponent = next_exponent;
+        const bool whole = valid == 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < G::NV; ++i) {
             const int c = i * kWave + lane;
             const int row = c / G::CPR;
-            const float unit = UnitOf(__shfl(t.exponent, 32 + row));
-            uint4 lo = Widen8<T>(t.v[i].x, t.v[i].y, unit);
-            uint4 hi = Widen8<T>(t.v[i].z, t.v[i].w, unit);
-            if (((t.valid >> row) & 1u) == 0) {  // weight 0, but the row may hold a NaN
-                lo = make_uint4(0, 0, 0, 0);
-                hi = lo;
+            const float unit = UnitOf(__shfl(exponent, 32 + row));
+            uint4 lo = Widen8<T>(v[i].x, v[i].y, unit);
+            uint4 hi = Widen8<T>(v[i].z, v[i].w, unit);
+            if (!whole) {  // rows that do not exist: weight 0, but they may hold a NaN
+                const uint32_t keep = (valid >> row) & 1u ? ~0u : 0u;
+                lo = make_uint4(lo.x & keep, lo.y & keep, lo.z & keep, lo.w & keep);
+                hi = make_uint4(hi.x & keep, hi.y & keep, hi.z & keep, hi.w & keep);
             }
             uint4* dst = reinterpret_cast<uint4*>(vs + row * G::RB + (((c % G::CPR) ^ VSwz<D>(row)) * 32));
             dst[0] = lo;
             dst[1] = hi;
         }
+        if (more) issue_v(next_row);
         floatx4 s[2];
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            const float unit = UnitOf(__shfl(t.exponent, 16 * rt + col));
+            const float unit = UnitOf(__shfl(exponent, 16 * rt + col));
             s[rt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < G::N16; ++j) {
-                const uint4 w = t.k16[rt][j];
+                const u32x4 w = k16[rt][j];
                 s[rt] = M::mma(__builtin_bit_cast(vec8, Widen8<T>(w.x, w.y, unit)), qb[2 * j], s[rt]);
                 s[rt] = M::mma(__builtin_bit_cast(vec8, Widen8<T>(w.z, w.w, unit)), qb[2 * j + 1], s[rt]);
             }
             if constexpr (G::N8) {
-                const uint2 w = t.k8[rt];
+                const u32x2 w = k8[rt];
                 s[rt] = M::mma(__builtin_bit_cast(vec8, Widen8<T>(w.x, w.y, unit)), qb[G::NK - 1], s[rt]);
             }
         }
+        if (more) issue_k();
         float sv[2][4];
         float mx = neg_inf();
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int tok = 16 * rt + 4 * grp + i;
-                const float x = ((t.valid >> tok) & 1u) ? s[rt][i] * scale2 : neg_inf();
+                float x = s[rt][i] * scale2;
+                if (!whole) x = ((valid >> (16 * rt + 4 * grp + i)) & 1u) ? x : neg_inf();
                 sv[rt][i] = x;
                 mx = fmaxf(mx, x);
             }
@@ -276,23 +290,16 @@ __global__ __launch_bounds__(kDecodeThreads) void decode8_kernel(const sca_decod
         __builtin_amdgcn_wave_barrier();
     };
 
-    // Tiles of this wave, two in flight; the page ids of the third are fetched behind them.
-    Dec8Tile<D> t0, t1;
     int tile = kWaveHeads ? 0 : wave;
-    int64_t row = row_of(tile < n_tiles ? tile : 0);
-    if (tile < n_tiles) issue(row, t0);
-    if (tile + TS < n_tiles) issue(row_of(tile + TS), t1);
-    row = row_of(tile + 2 * TS);
-    while (tile < n_tiles) {
-        compute(t0);
-        if (tile + 2 * TS < n_tiles) issue(row, t0);
-        row = row_of(tile + 3 * TS);
-        tile += TS;
-        if (tile >= n_tiles) break;
-        compute(t1);
-        if (tile + 2 * TS < n_tiles) issue(row, t1);
-        row = row_of(tile + 3 * TS);
-        tile += TS;
+    if (tile < n_tiles) {
+        issue_v(row_of(tile));
+        issue_k();
+    }
+    int row = row_of(tile + TS);
+    for (; tile < n_tiles; tile += TS) {
+        const int now = row;
+        row = row_of(tile + 2 * TS);
+        compute(tile + TS < n_tiles, now);
     }
 
     if constexpr (M::kScale != 1.0f) {
@@ -450,7 +457,9 @@ int ValidateDecode8(const sca_decode8_params* p8) {
                         "decode8: invalid heads (H_q=" + std::to_string(p->num_heads) +
                             ", H_kv=" + std::to_string(p->num_kv_heads) + ") or batch");
     }
-    if (p->seq_kv < 0) return SetError(SCA_E_SHAPE_MISMATCH, "decode8: seq_kv < 0");
+    if (p->seq_kv < 0 || p->seq_kv > 0x7fffffff - 4096) {
+        return SetError(SCA_E_SEQ_TOO_LONG, "decode8: seq_kv=" + std::to_string(p->seq_kv));
+    }
     if (p->dtype != SCA_DTYPE_F16 && p->dtype != SCA_DTYPE_BF16) {
         return SetError(SCA_E_UNSUPPORTED_DTYPE,
                         "decode8: queries are fp16 or bf16; dtype id " + std::to_string(p->dtype));
@@ -463,9 +472,9 @@ int ValidateDecode8(const sca_decode8_params* p8) {
     }
     if (!Aligned16(p->q) || !Aligned16(p->k) || !Aligned16(p->v) || !Aligned16(p->out) || p->q_sb % 8 ||
         p->q_sh % 8 || p->o_sb % 8 || p->o_sh % 8 || p->k_sh % 16 || p->k_ss % 16 || p->v_sh % 16 ||
-        p->v_ss % 16) {
+        p->v_ss % 16 || p->k_ss < 0 || p->k_ss > 0x7fffffff || p->v_ss < 0 || p->v_ss > 0x7fffffff) {
         return SetError(SCA_E_LAYOUT_MISMATCH,
-                        "decode8: pointers must be 16 B aligned and strides multiples of 16 B");
+                        "decode8: pointers must be 16 B aligned, strides multiples of 16 B, row strides from 0 to 2^31");
     }
     if (p->slot_waves != 0 && p->slot_waves != 1 && p->slot_waves != kDecodeWaves) {
         return SetError(SCA_E_SHAPE_MISMATCH,
