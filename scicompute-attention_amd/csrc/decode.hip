@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "decode_common.hpp"
+#include "decode_order.hpp"
 #include "sca_device.hpp"
 
 namespace sca_hip {

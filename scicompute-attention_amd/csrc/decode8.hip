@@ -21,6 +21,7 @@
 #include <string>
 
 #include "decode_common.hpp"
+#include "decode_order.hpp"
 #include "e4m3.hpp"
 #include "sca_device.hpp"
 
@@ -457,7 +458,8 @@ int ValidateDecode8(const sca_decode8_params* p8) {
                         "decode8: invalid heads (H_q=" + std::to_string(p->num_heads) +
                             ", H_kv=" + std::to_string(p->num_kv_heads) + ") or batch");
     }
-    if (p->seq_kv < 0 || p->seq_kv > 0x7fffffff - 4096) {
+    if (p->seq_kv < 0) return SetError(SCA_E_SHAPE_MISMATCH, "decode8: seq_kv < 0");
+    if (p->seq_kv > 0x7fffffff - 4096) {
         return SetError(SCA_E_SEQ_TOO_LONG, "decode8: seq_kv=" + std::to_string(p->seq_kv));
     }
     if (p->dtype != SCA_DTYPE_F16 && p->dtype != SCA_DTYPE_BF16) {

@@ -1,6 +1,5 @@
 // Shared pieces of the decode kernels over 16/32-bit pages (decode.hip) and over 8-bit pages
-// (decode8.hip): element traits, MFMA wrappers, the split range, the longest-first schedule and the
-// log-sum-exp combine.
+// (decode8.hip): element traits, MFMA wrappers, the split range and the log-sum-exp combine.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -242,25 +241,6 @@ template <int D>
 __device__ __forceinline__ int VSwz(int t) {
     constexpr int kStart = (D / 16) % 8;
     return kStart == 0 ? (t & 7) : kStart == 4 ? ((t >> 1) & 3) : ((t >> 2) & 1);
-}
-
-// Longest-first schedule of ragged batches larger than kRankBatch: entry r of `order` is
-// (b, len_b) for the sequence of rank r (descending length, ties by index). The MFMA kernels
-// take the sequence of grid row z from entry z, so the longest sequences are dispatched first.
-constexpr int kMaxOrderedBatch = 8192;
-
-__global__ __launch_bounds__(256) void decode_order_kernel(const int32_t* seq_lens, int batch,
-                                                           int32_t* order) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b >= batch) return;
-    const int mine = seq_lens[b];
-    int rank = 0;
-    for (int j = 0; j < batch; ++j) {
-        const int other = seq_lens[j];
-        rank += (other > mine) | ((other == mine) & (j < b));
-    }
-    order[2 * rank] = b;
-    order[2 * rank + 1] = mine;
 }
 
 bool Aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }

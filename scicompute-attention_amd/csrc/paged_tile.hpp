@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     const PagedSeq& sq = u.seq;
     const int rows = sq.q_count * p.group;
     const int diag = p.causal ? sq.keys - sq.q_count : 0;
-    const int visible = VisibleKeys(sq, u.tile, p.group, p.causal != 0);
+    const int visible = VisibleKeys(sq, u.tile, kPagedRows, p.group, p.causal != 0);
     const int all_tiles = (visible + BN - 1) / BN;
     int first = 0, n_tiles = all_tiles;
     if (sq.splits > 1) SplitRange(all_tiles, sq.splits, u.split, &first, &n_tiles);

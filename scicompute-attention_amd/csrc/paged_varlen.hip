@@ -1,6 +1,6 @@
 // Attention of ragged chunks of new tokens over paged KV: the plan of a call (units, key splits, the
 // launches' sequence lists), the merge of key splits, the checks and the C entry points. The kernels
-// are in paged_tile.hpp; paged_varlen.hpp describes rows, units and splits.
+// are in paged_tile.hpp and paged_few.hpp; paged_varlen.hpp describes rows, units and splits.
 
 #include <hip/hip_runtime.h>
 
@@ -70,67 +70,89 @@ bool Aligned(const void* ptr, uintptr_t bytes) {
     return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0;
 }
 
-int KeysPerTile(int64_t head_dim) { return head_dim <= 128 ? 64 : 32; }
+// The kernels that serve a call: tiles of 128 rows, or the few-token kernel's 16 or 32.
+enum Kind { kTile, kFew16, kFew32 };
 
-// One sequence of a call, in the order of the launches.
-struct Planned {
-    PagedSeq seq;
-    int64_t tiles;  // key tiles of its last row tile
+struct Launch {
+    Kind kind;
+    PagedSeqs seqs;
+    int64_t units;
+    int64_t combine_rows;  // most (KV head, row) pairs of a split sequence; 0: no merge
 };
 
 struct Plan {
-    std::vector<PagedSeqs> launches;
-    std::vector<int64_t> units;
-    std::vector<int64_t> combine_rows;  // most (KV head, row) pairs of a split sequence; 0: no merge
-    int64_t states = 0;                 // most states a launch leaves
+    std::vector<Launch> launches;
+    int64_t states = 0;  // most states a launch leaves
 };
 
-// Workgroups that the GPU holds at once.
-int64_t Resident(int64_t head_dim) {
-    return static_cast<int64_t>(CuCount()) * (head_dim <= 96 ? 2 : 1);
+// Sequences of up to 32 packed rows take the few-token kernel (16 at head_dim 256, where two column
+// groups of O do not fit the registers).
+Kind KindFor(const sca_paged_varlen_params& p, int64_t rows) {
+    if (rows <= 16) return kFew16;
+    if (rows <= 32) return p.head_dim <= 192 ? kFew32 : kFew16;
+    return kTile;
 }
 
-// `may_split`: states may go to `most_states` of scratch.
-Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
+int RowsPerTile(Kind kind) { return kind == kTile ? kPagedRows : kind == kFew32 ? 32 : 16; }
+
+// Keys that a workgroup takes in one step.
+int KeysPerStep(Kind kind, int64_t head_dim) { return kind != kTile ? 128 : head_dim <= 128 ? 64 : 32; }
+
+// Workgroups that the GPU holds at once.
+int64_t Resident(Kind kind, const sca_paged_varlen_params& p) {
+    const int d = static_cast<int>(p.head_dim);
+    const int on_cu = kind == kTile ? (d <= 128 ? 2 : 1) : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
+    return static_cast<int64_t>(CuCount()) * on_cu;
+}
+
+// The launches of one kind, appended to `plan`. States of split keys may go to `most_states` of scratch.
+void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, Plan* plan) {
+    struct Entry {
+        PagedSeq seq;
+        int64_t steps;  // of its last row tile
+    };
     const int64_t group = p.num_heads / p.num_kv_heads;
-    const int bn = KeysPerTile(p.head_dim);
-    std::vector<Planned> list;
-    int64_t work = 0;   // key tiles of all units
+    const int64_t rows_per_tile = RowsPerTile(kind);
+    const int64_t keys = KeysPerStep(kind, p.head_dim);
+    std::vector<Entry> list;
+    int64_t work = 0;  // steps of all units
     for (int64_t s = 0; s < p.num_seqs; ++s) {
         const int64_t n = p.cu_seqlens_q[s + 1] - p.cu_seqlens_q[s];
-        if (n == 0) continue;
-        Planned e{};
+        if (n == 0 || KindFor(p, n * group) != kind) continue;
+        Entry e{};
         e.seq.q_first = p.cu_seqlens_q[s];
         e.seq.q_count = static_cast<int32_t>(n);
         e.seq.keys = p.kv_lens[s];
         e.seq.table_row = p.table_rows != nullptr ? p.table_rows[s] : static_cast<int32_t>(s);
         e.seq.splits = 1;
-        e.seq.row_tiles = static_cast<int32_t>((n * group + kPagedRows - 1) / kPagedRows);
-        e.tiles = (p.kv_lens[s] + bn - 1) / bn;
+        e.seq.row_tiles = static_cast<int32_t>((n * group + rows_per_tile - 1) / rows_per_tile);
+        e.steps = (p.kv_lens[s] + keys - 1) / keys;
         // (causal: the row tiles of new tokens see fewer keys; their mean serves the estimate)
-        const int64_t mean = p.causal ? std::max<int64_t>(1, e.tiles - std::min<int64_t>(n, p.kv_lens[s]) / (2 * bn))
-                                      : e.tiles;
+        const int64_t mean =
+            p.causal ? std::max<int64_t>(1, e.steps - std::min<int64_t>(n, p.kv_lens[s]) / (2 * keys)) : e.steps;
         work += p.num_kv_heads * e.seq.row_tiles * mean;
         list.push_back(e);
     }
-    // Key splits: every unit at most the share of one resident workgroup (and at least kLeastTiles), for
-    // the sequences where that saves kWorthTiles steps of the longest unit: the states' traffic and the
-    // merge's launch cost about as much as those.
-    constexpr int64_t kLeastTiles = 4, kWorthTiles = 8;
-    const int64_t span = std::max<int64_t>(kLeastTiles, (work + Resident(p.head_dim) - 1) / Resident(p.head_dim));
-    for (Planned& e : list) {
-        if (most_states > 0 && e.tiles - span >= kWorthTiles) {
-            e.seq.splits = static_cast<int32_t>(std::min<int64_t>(64, (e.tiles + span - 1) / span));
+    if (list.empty()) return;
+    // Key splits: every unit at most the share of one resident workgroup, for the sequences where that
+    // saves enough steps of the longest unit to pay for the states' traffic and the merge's launch (a
+    // step takes about 1 us in either kernel, those 5 us and more).
+    const int64_t least = kind == kTile ? 4 : 1, worth = kind == kTile ? 8 : 3;
+    const int64_t resident = Resident(kind, p);
+    const int64_t span = std::max(least, (work + resident - 1) / resident);
+    for (Entry& e : list) {
+        if (most_states > 0 && e.steps - span >= worth) {
+            e.seq.splits = static_cast<int32_t>(std::min<int64_t>(64, (e.steps + span - 1) / span));
         }
     }
     // Longest units first.
-    std::stable_sort(list.begin(), list.end(), [](const Planned& a, const Planned& b) {
-        return a.tiles * b.seq.splits > b.tiles * a.seq.splits;
+    std::stable_sort(list.begin(), list.end(), [](const Entry& a, const Entry& b) {
+        return a.steps * b.seq.splits > b.steps * a.seq.splits;
     });
-    Plan plan;
     for (size_t at = 0; at < list.size(); at += kPagedSeqs) {
-        PagedSeqs seqs{};
-        int64_t units = 0, states = 0, combine = 0;
+        Launch launch{};
+        launch.kind = kind;
+        int64_t states = 0;
         for (size_t i = at; i < std::min(list.size(), at + kPagedSeqs); ++i) {
             PagedSeq q = list[i].seq;
             const int64_t rows = q.q_count * group * p.num_kv_heads;
@@ -138,28 +160,42 @@ Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
             q.state_base = static_cast<int32_t>(states);
             if (q.splits > 1) {
                 states += rows * q.splits;
-                combine = std::max(combine, rows);
+                launch.combine_rows = std::max(launch.combine_rows, rows);
             }
-            units += static_cast<int64_t>(q.row_tiles) * q.splits * p.num_kv_heads;
-            q.unit_end = static_cast<int32_t>(std::min<int64_t>(units, 0x7fffffff));
-            seqs.seq[seqs.count++] = q;
+            launch.units += static_cast<int64_t>(q.row_tiles) * q.splits * p.num_kv_heads;
+            q.unit_end = static_cast<int32_t>(launch.units);  // (Validate bounds the units)
+            launch.seqs.seq[launch.seqs.count++] = q;
         }
-        plan.launches.push_back(seqs);
-        plan.units.push_back(units);
-        plan.combine_rows.push_back(combine);
-        plan.states = std::max(plan.states, states);
+        plan->states = std::max(plan->states, states);
+        plan->launches.push_back(launch);
     }
+}
+
+// Long chunks first: the few-token launches fill the GPU behind them.
+Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
+    Plan plan;
+    for (Kind kind : {kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
     return plan;
 }
 
 int64_t StateBytes(int64_t head_dim) { return 4 * (head_dim + 2); }
 
+template <typename E, int D, bool kHeld8>
+int LaunchKind(const PagedArgs& a, const Launch& l, hipStream_t s) {
+    const int units = static_cast<int>(l.units);
+    if (l.kind == kTile) return LaunchPagedTile<E, D, kHeld8>(a, l.seqs, units, s);
+    if constexpr (D <= 192) {
+        if (l.kind == kFew32) return LaunchPagedFew<E, D, kHeld8, 2>(a, l.seqs, units, s);
+    }
+    return LaunchPagedFew<E, D, kHeld8, 1>(a, l.seqs, units, s);
+}
+
 template <typename E>
-int LaunchTile(const PagedArgs& a, const PagedSeqs& seqs, int units, int64_t head_dim, hipStream_t s) {
+int LaunchOne(const PagedArgs& a, const Launch& l, int64_t head_dim, hipStream_t s) {
     const bool held8 = a.k_exp != nullptr;
     switch (head_dim) {
 #define SCA_CASE(D) \
-    case D: return held8 ? LaunchPagedTile<E, D, true>(a, seqs, units, s) : LaunchPagedTile<E, D, false>(a, seqs, units, s);
+    case D: return held8 ? LaunchKind<E, D, true>(a, l, s) : LaunchKind<E, D, false>(a, l, s);
         SCA_CASE(32)
         SCA_CASE(64)
         SCA_CASE(96)
@@ -190,14 +226,14 @@ int Run(const sca_paged_varlen_params& p, const Plan& plan, void* scratch, hipSt
     while ((int64_t{1} << a.block_shift) < p.block_size) ++a.block_shift;
     a.causal = p.causal;
     a.scale = p.scale;
-    for (size_t i = 0; i < plan.launches.size(); ++i) {
-        int rc = LaunchTile<E>(a, plan.launches[i], static_cast<int>(plan.units[i]), p.head_dim, s);
+    for (const Launch& l : plan.launches) {
+        int rc = LaunchOne<E>(a, l, p.head_dim, s);
         if (rc != 0) return rc;
-        if (plan.combine_rows[i] == 0) continue;
-        const int64_t threads = plan.combine_rows[i] * (p.head_dim / 4);
+        if (l.combine_rows == 0) continue;
+        const int64_t threads = l.combine_rows * (p.head_dim / 4);
         const dim3 grid(static_cast<unsigned>((threads + kCombineThreads - 1) / kCombineThreads),
-                        static_cast<unsigned>(plan.launches[i].count));
-        hipLaunchKernelGGL((paged_combine_kernel<E>), grid, dim3(kCombineThreads), 0, s, a, plan.launches[i],
+                        static_cast<unsigned>(l.seqs.count));
+        hipLaunchKernelGGL((paged_combine_kernel<E>), grid, dim3(kCombineThreads), 0, s, a, l.seqs,
                            static_cast<uint32_t>(p.head_dim));
         rc = CheckLaunch("paged_combine_kernel", s);
         if (rc != 0) return rc;
@@ -254,6 +290,9 @@ int Validate(const sca_paged_varlen_params* p, bool pointers) {
         p->v_ss % ve || p->v_sh % ve) {
         return fail(SCA_E_LAYOUT_MISMATCH, "strides must be multiples of 16 B");
     }
+    if (p->k_ss < 0 || p->k_ss >= (1LL << 30) || p->v_ss < 0 || p->v_ss >= (1LL << 30)) {
+        return fail(SCA_E_LAYOUT_MISMATCH, "K and V row strides must be below 2^30 and not negative");
+    }
     const int64_t group = p->num_heads / p->num_kv_heads;
     int64_t units = 0;
     if (p->cu_seqlens_q[0] < 0) return fail(SCA_E_SHAPE_MISMATCH, "cu_seqlens_q starts below 0");
@@ -274,7 +313,7 @@ int Validate(const sca_paged_varlen_params* p, bool pointers) {
             return fail(SCA_E_SEQ_TOO_LONG, "sequence " + std::to_string(s) + " of " + std::to_string(n) +
                                                 " new tokens and " + std::to_string(p->kv_lens[s]) + " keys");
         }
-        units += (n * group + kPagedRows - 1) / kPagedRows * p->num_kv_heads;
+        units += (n * group + 15) / 16 * p->num_kv_heads;  // (no kernel has fewer rows to a unit)
     }
     if (units > 0x7fffffffLL / 64) {
         return fail(SCA_E_SEQ_TOO_LONG, "grid of " + std::to_string(units) + " row tiles exceeds the launch limit");

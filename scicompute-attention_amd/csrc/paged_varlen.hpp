@@ -2,7 +2,7 @@
 //
 // Rows. The query heads of one KV head read the same keys, so their rows share row tiles: packed row
 // R of a (sequence, KV head) is new token R / group of head R % group. A chunk of 32 tokens with four
-// heads a group is one 128-row tile; a single token fills `group` rows of its tile.
+// heads a group is one 128-row tile. Sequences of few rows go to a kernel with tiles of 16 or 32 rows.
 // Units. A workgroup takes one unit: (sequence, row tile, key split, KV head). The sequences of a
 // launch are listed in the kernel's arguments (PagedSeq), at most kPagedSeqs of them; more go out in
 // further launches. So nothing is uploaded, and a captured launch keeps its own list.
@@ -22,6 +22,14 @@ namespace sca_hip {
 
 constexpr int kPagedRows = 128;   // packed rows per workgroup
 constexpr int kPagedSeqs = 112;   // sequences per launch: 32 B each, below 4 KB of arguments
+
+// Workgroups of the few-token kernel that a CU holds: O and Q of its column groups and a tile's K and V
+// in registers (as built; more would spill).
+constexpr int FewResident(int head_dim, bool held8, int column_groups) {
+    const int need = column_groups * (head_dim / 16 * 4 + head_dim / 32 * 4) +
+                     (held8 ? head_dim / 4 : head_dim / 2) + 70;
+    return need <= 96 ? 5 : need <= 128 ? 4 : need <= 168 ? 3 : need <= 256 ? 2 : 1;
+}
 
 struct PagedSeq {
     int32_t unit_end;    // units of this and all earlier sequences of the launch
@@ -61,6 +69,8 @@ static_assert(sizeof(PagedArgs) + sizeof(PagedSeqs) <= 4096, "kernel arguments")
 // Launchers, instantiated in the file of their kernel; `units` workgroups.
 template <typename E, int D, bool kHeld8>
 int LaunchPagedTile(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_tile.hpp
+template <typename E, int D, bool kHeld8, int NC>
+int LaunchPagedFew(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_few.hpp
 
 namespace {
 
@@ -95,9 +105,10 @@ __device__ __forceinline__ PagedUnit FindUnit(const PagedSeqs& seqs, int kv_head
 }
 
 // Keys that the rows of a tile see at most: all, or up to its last token's own position.
-__device__ __forceinline__ int VisibleKeys(const PagedSeq& s, int tile, int group, bool causal) {
+__device__ __forceinline__ int VisibleKeys(const PagedSeq& s, int tile, int tile_rows, int group,
+                                           bool causal) {
     if (!causal) return s.keys;
-    const int last_row = min((tile + 1) * kPagedRows, s.q_count * group) - 1;
+    const int last_row = min((tile + 1) * tile_rows, s.q_count * group) - 1;
     const int last = static_cast<int>(static_cast<uint32_t>(last_row) / static_cast<uint32_t>(group));
     return max(0, min(s.keys, last + s.keys - s.q_count + 1));
 }
