@@ -38,12 +38,25 @@
 namespace sca_hip {
 namespace {
 
-// kMode: plain, packed varlen, or cut (rows packed and / or keys split: SplitArgs).
-enum WideMode { kPlain, kPackedVarlen, kCut };
+// kMode: plain, packed varlen, cut (rows packed and / or keys split: SplitArgs), or paged (PagedJob:
+// packed rows of one sequence over the pages of its keys).
+enum WideMode { kPlain, kPackedVarlen, kCut, kPaged };
+
+// A workgroup's share of a launch over paged KV (kPaged): packed rows of one row tile and KV head, and
+// a range of key tiles. Pages of at least 16 tokens.
+struct PagedJob {
+    const int32_t* table;   // the sequence's row of the page table
+    int64_t max_blocks, num_blocks;
+    int block_shift;
+    int q_first, q_count, keys;
+    int tile, split, splits, h_kv;
+    int64_t state;          // splits > 1: the state of packed row 0 of this (split, KV head)
+};
 
 template <typename E, int D, bool kCausal, WideMode kMode, Denominator kDen>
-__global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel(
-    const sca_flash_params p, int num_q_tiles, const VarlenArgs vl, const SplitArgs sp) {
+__device__ __forceinline__ void FlashWide(const sca_flash_params& p, int num_q_tiles,
+                                          const VarlenArgs& vl, const SplitArgs& sp,
+                                          const PagedJob& job) {
     using G = WideGeom<D>;
     using M = Mfma<E>;
     using A = MfmaAsm<E>;
@@ -52,6 +65,10 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
     constexpr int BM = G::BM;
     constexpr int RB = G::ROW_BYTES;
     constexpr bool kVarlen = kMode == kPackedVarlen;
+    constexpr int kPagedRowsPerWave = BN / G::WAVES;  // 16
+    // log2 headroom of the weights over paged KV: fp16 weights keep all their bits down to 2^-21 of the
+    // row's largest and stay finite, at most 2^(7 + kRescaleSlack).
+    constexpr float kBias = kMode == kPaged && std::is_same_v<E, F16> ? 7.0f : 0.0f;
 
     extern __shared__ __align__(16) uint8_t lds8[];
     const int tid = threadIdx.x;
@@ -62,13 +79,18 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
     const int rg = wave & 1;   // row group: rows 64*rg .. +64 of the row tile
     const int kq = wave >> 1;  // key half: keys 32*kq .. +32 of every key tile
 
-    const int pack = kMode == kCut ? sp.pack : 1;
-    const int splits = kMode == kCut ? sp.splits : 1;
-    int tile_linear, b_, unit;
-    XcdOrder(p, static_cast<uint32_t>(p.num_heads) / static_cast<uint32_t>(pack), &tile_linear, &b_,
-             &unit);
+    const int pack = kMode == kCut || kMode == kPaged ? sp.pack : 1;
+    const int splits = kMode == kCut ? sp.splits : kMode == kPaged ? job.splits : 1;
+    int tile_linear = 0, b_ = 0, unit = 0;
     int split = 0;
-    if (splits > 1) {
+    if constexpr (kMode == kPaged) {
+        unit = job.h_kv;
+        split = job.split;
+    } else {
+        XcdOrder(p, static_cast<uint32_t>(p.num_heads) / static_cast<uint32_t>(pack), &tile_linear, &b_,
+                 &unit);
+    }
+    if (kMode != kPaged && splits > 1) {
         split = tile_linear % splits;
         tile_linear /= splits;
     }
@@ -91,6 +113,13 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         seq_q = vl.cu_q[seq + 1] - static_cast<int>(tok_q);
         seq_kv = vl.cu_kv[seq + 1] - static_cast<int>(tok_kv);
         diag = kCausal ? seq_kv - seq_q : 0;
+    }
+    if constexpr (kMode == kPaged) {
+        qt = job.tile;
+        tok_q = job.q_first;
+        seq_q = job.q_count;
+        seq_kv = job.keys;
+        diag = static_cast<int>(p.diagonal);  // (keys - new tokens, or so large that every key is seen)
     }
     const float scale2 = p.scale * kLog2e;
     const float inv_scale2 = 1.0f / scale2;
@@ -124,7 +153,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         // Key tiles [first, first + count): the keys, the causal diagonal and K/V start there.
         int first, count;
         SplitRange(n_tiles, splits, split, &first, &count);
-        if (count == 0) {  // fewer key tiles than splits: a state that the merge skips
+        if (kMode != kPaged && count == 0) {  // fewer key tiles than splits: a state that the merge skips
             if (hh == 0) {
                 const int r = kq;  // each of the two waves of a row group covers one subtile
                 const int q = r == 0 ? qi[0] : qi[1];
@@ -142,13 +171,15 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         diag -= first * BN;
         n_tiles = count;
         n_plain = max(0, min(n_plain - first, count));
+        // (paged: a range without keys runs through with every score masked, and leaves zeros)
+        if (kMode == kPaged && count == 0) seq_kv = 0;
     }
 
     // ---- DMA (buffer resources bounded at the sequence's last row) ----
     const uint8_t* k_bytes = reinterpret_cast<const uint8_t*>(
-        static_cast<const uint16_t*>(p.k) + b * p.k_sb + h_kv * p.k_sh + tok_kv * p.k_ss);
+        static_cast<const uint16_t*>(p.k) + b * p.k_sb + h_kv * p.k_sh + (kMode == kPaged ? 0 : tok_kv) * p.k_ss);
     const uint8_t* v_bytes = reinterpret_cast<const uint8_t*>(
-        static_cast<const uint16_t*>(p.v) + b * p.v_sb + h_kv * p.v_sh + tok_kv * p.v_ss);
+        static_cast<const uint16_t*>(p.v) + b * p.v_sb + h_kv * p.v_sh + (kMode == kPaged ? 0 : tok_kv) * p.v_ss);
     const int k_row_bytes = static_cast<int>(p.k_ss) * 2;
     const int v_row_bytes = static_cast<int>(p.v_ss) * 2;
     const int k_records = (seq_kv - 1) * k_row_bytes + RB;
@@ -159,9 +190,60 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         const int P = (wave * G::IPW + i) * kWave + lane;
         const int row = P / G::CPR;
         const int pos = P % G::CPR;
-        dma_koff[i] = row * k_row_bytes + (pos ^ SwzK<D>(row)) * 16;
-        dma_voff[i] = row * v_row_bytes + (pos ^ SwzV<D>(row)) * 16;
+        const int from = kMode == kPaged ? row - wave * kPagedRowsPerWave : row;  // paged: in the wave's rows
+        dma_koff[i] = from * k_row_bytes + (pos ^ SwzK<D>(row)) * 16;
+        dma_voff[i] = from * v_row_bytes + (pos ^ SwzV<D>(row)) * 16;
     }
+    // Paged: a wave copies 16 rows of every tile, which one page holds. Their page id comes through the
+    // scalar cache, a step ahead of its use; a buffer resource of their own, bounded at the rows that
+    // exist, makes the rest read as zeros (keys past the end, unmapped pages).
+    // All without branches, in 32 bits (keys and pool rows are below 2^31).
+    const int key0 = static_cast<int>(tok_kv);  // of tile 0
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(job.table);
+    const uint32_t num_blocks = static_cast<uint32_t>(job.num_blocks);
+    // Keys that the table's row covers; the last entry that is read.
+    const int mapped = static_cast<int>(
+        min(static_cast<int64_t>(job.keys), job.max_blocks << job.block_shift));
+    const int last_page = max(0, mapped - 1) >> job.block_shift;
+    auto page_id = [&](int key) __attribute__((always_inline)) -> int {
+        return table[min(key >> job.block_shift, last_page)];
+    };
+    struct Rows {
+        uint32_t row;  // pool row
+        int count;     // rows that exist, from there (0 or less: none)
+    };
+    auto rows_of = [&](int t, int id) __attribute__((always_inline)) -> Rows {
+        const int key = key0 + t * BN + wave * kPagedRowsPerWave;
+        const bool ok = static_cast<uint32_t>(id) < num_blocks;  // (negative ids are large ones)
+        const uint32_t row = (static_cast<uint32_t>(id) << job.block_shift) +
+                             (static_cast<uint32_t>(key) & ((1u << job.block_shift) - 1));
+        return {ok ? row : 0, ok ? min(kPagedRowsPerWave, mapped - key) : 0};
+    };
+    // Whether tile t has keys on pages that are not mapped, among this wave's half: bit g for keys
+    // 16 g .. + 16 of it. (Keys past the end are masked by their number.)
+    auto holes_of = [&](int t, int id0, int id1) __attribute__((always_inline)) -> int {
+        const int key = key0 + t * BN + 32 * kq;
+        const int a = static_cast<uint32_t>(id0) >= num_blocks || key >= mapped ? 1 : 0;
+        const int b = static_cast<uint32_t>(id1) >= num_blocks || key + 16 >= mapped ? 2 : 0;
+        return a | b;
+    };
+    auto half_id = [&](int t, int g) __attribute__((always_inline)) -> int {
+        return page_id(key0 + t * BN + 32 * kq + 16 * g);
+    };
+    auto own_id = [&](int t) __attribute__((always_inline)) -> int {
+        return page_id(key0 + t * BN + wave * kPagedRowsPerWave);
+    };
+    auto dma_rows = [&](bool is_k, const Rows& r, int slot, int i) __attribute__((always_inline)) {
+        const int row_bytes = is_k ? k_row_bytes : v_row_bytes;
+        const uint8_t* base = (is_k ? k_bytes : v_bytes) + static_cast<uint64_t>(r.row) * static_cast<uint32_t>(row_bytes);
+        const int records = r.count > 0 ? (r.count - 1) * row_bytes + RB : 0;
+        uint8_t* dst = lds8 + (is_k ? 0 : G::V_BASE) + slot * G::TILE_BYTES + wave * G::IPW * 1024;
+        DmaToLds(base, records, dst + i * 1024, is_k ? dma_koff[i] : dma_voff[i], 0);
+    };
+    auto dma_tile = [&](bool is_k, const Rows& r, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < G::IPW; ++i) dma_rows(is_k, r, slot, i);
+    };
     auto issue_k = [&](int slot, int t) __attribute__((always_inline)) {
         uint8_t* dst = lds8 + slot * G::TILE_BYTES + wave * G::IPW * 1024;
         const uint32_t off = static_cast<uint32_t>(t * BN * k_row_bytes);
@@ -263,14 +345,14 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
     };
 
     // Masking of S^T subtile r of key tile t (uniform `masked`), and the lane's local maximum.
-    auto mask_max = [&](floatx16& sr, int r, int t, bool masked) __attribute__((always_inline)) -> float {
+    auto mask_max = [&](floatx16& sr, int r, int t, bool masked, int holes) __attribute__((always_inline)) -> float {
         if (masked) {
             const int kbase = t * BN + 32 * kq + 4 * hh;
             const int lim = kCausal ? min(seq_kv - 1, qi[r] + diag) : seq_kv - 1;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = kbase + 8 * (i / 4) + (i % 4);
-                sr[i] = key > lim ? neg_inf() : sr[i];
+                sr[i] = key > lim || (kMode == kPaged && ((holes >> (i / 8)) & 1)) ? neg_inf() : sr[i];
             }
         }
         return Max16(sr);
@@ -283,8 +365,8 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
 #pragma unroll
         for (int r = 0; r < G::RT; ++r) {
             const float cmax = HalfMax(lmv[r]) * scale2;  // row maximum, log2 units
-            const bool grow = cmax > rs[r].m + kRescaleSlack;
-            const float m_new = grow ? cmax : rs[r].m;
+            const bool grow = cmax > rs[r].m + (kRescaleSlack + kBias);
+            const float m_new = grow ? cmax - kBias : rs[r].m;
             const float alpha = grow ? fast_exp2(rs[r].m - m_new) : 1.0f;  // 0 when m was -inf
             rs[r].m = m_new;
             rs[r].l *= alpha;
@@ -298,7 +380,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
                 PinAgpr(o[r][dt]);
             }
             Fence();
-            rs[r].thr = (m_new + kRescaleSlack) * inv_scale2;
+            rs[r].thr = (m_new + (kRescaleSlack + kBias)) * inv_scale2;
             rs[r].neg_mu = (m_new == neg_inf()) ? 0.0f : -m_new;
         }
         asm volatile("s_nop 4");
@@ -306,7 +388,23 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
 
     // ---- prologue: K(0..3), V(0..2) in flight; S(0), its maxima and rescale; K(1) and V(0)
     //      fragments read for step 0; K(2) and V(1) landed before step 0 ----
-    issue_k(0, 0);
+    // (paged: the rows and holes of the tiles that the prologue and the first step use)
+    Rows rows_k{0, 0}, rows_v{0, 0};  // of the step's K and V tiles
+    int id_own = 0, id_half0 = 0, id_half1 = 0, holes = 0;
+    Rows rows0{0, 0}, rows1{0, 0}, rows2{0, 0};
+    if constexpr (kMode == kPaged) {
+        const int i0 = own_id(0), i1 = own_id(1), i2 = own_id(2), i3 = own_id(3);
+        const int a0 = half_id(0, 0), a1 = half_id(0, 1);
+        id_own = own_id(4);
+        rows0 = rows_of(0, i0);
+        rows1 = rows_of(1, i1);
+        rows2 = rows_of(2, i2);
+        rows_v = rows_of(3, i3);
+        holes = holes_of(0, a0, a1);
+        dma_tile(true, rows0, 0);
+    } else {
+        issue_k(0, 0);
+    }
     // Q fragments (B operand of S^T = K Q^T): subtile r, k-step ks. Rows past seq_q repeat the last
     // one (their results are not stored). Requested behind K(0) and pinned only after the other
     // tiles' DMAs are issued, so that nothing waits for them but the first QK.
@@ -321,12 +419,21 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             qf[r][ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const uint4*>(q_row + 16 * ks));
         }
     }
-    issue_k(1, 1);
-    issue_v(0, 0);
-    issue_k(2, 2);
-    issue_v(1, 1);
-    issue_k(3, 3);
-    issue_v(2, 2);
+    if constexpr (kMode == kPaged) {
+        dma_tile(true, rows1, 1);
+        dma_tile(false, rows0, 0);
+        dma_tile(true, rows2, 2);
+        dma_tile(false, rows1, 1);
+        dma_tile(true, rows_v, 3);
+        dma_tile(false, rows2, 2);
+    } else {
+        issue_k(1, 1);
+        issue_v(0, 0);
+        issue_k(2, 2);
+        issue_v(1, 1);
+        issue_k(3, 3);
+        issue_v(2, 2);
+    }
 #pragma unroll
     for (int r = 0; r < G::RT; ++r) {
 #pragma unroll
@@ -350,8 +457,9 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         // The first maxima; O and l are zero, so nothing is rescaled.
 #pragma unroll
         for (int r = 0; r < G::RT; ++r) {
-            rs[r].m = HalfMax(mask_max(s0[r], r, 0, n_plain == 0)) * scale2;
-            rs[r].thr = (rs[r].m + kRescaleSlack) * inv_scale2;
+            const bool masked = n_plain == 0 || (kMode == kPaged && holes != 0);
+            rs[r].m = HalfMax(mask_max(s0[r], r, 0, masked, holes)) * scale2 - kBias;
+            rs[r].thr = (rs[r].m + (kRescaleSlack + kBias)) * inv_scale2;
             rs[r].neg_mu = (rs[r].m == neg_inf()) ? 0.0f : -rs[r].m;
         }
     }
@@ -385,7 +493,19 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
         // end runs too (its scores are all masked): merging "computed" and "not computed" scores
         // would make the compiler copy MFMA results it does not know to be in flight.
         const bool next_ok = !kMaskable || D > 128 || j + 1 < n_tiles;
-        const bool next_masked = kMaskable && j + 1 >= n_plain;
+        int next_holes = 0;
+        if constexpr (kMode == kPaged) {
+            // The page ids asked for a step ago, and the next ones: the scalar loads are back before the
+            // step's last wait, so that their use costs none.
+            rows_k = rows_of(j + 4, id_own);
+            id_own = own_id(j + 5);
+            if constexpr (kMaskable) {
+                next_holes = holes_of(j + 1, id_half0, id_half1);
+                id_half0 = half_id(j + 2, 0);
+                id_half1 = half_id(j + 2, 1);
+            }
+        }
+        const bool next_masked = kMaskable && (j + 1 >= n_plain || (kMode == kPaged && next_holes != 0));
         uint32_t pw[G::RT][8];
         // The VALU operations that turn S(j) subtile r into P, in place (SoftmaxOp); op(r, n) runs
         // the n-th. (Unrounded sums use v_add: a v_dot2 issued between MFMAs does not overlap with
@@ -434,7 +554,11 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             if (n >= 2 * G::IPW || i / kSpacing >= kDmaPerRegion) return;
             const bool is_k = n < G::IPW;
             if (kMaskable && (is_k ? j + 4 >= n_tiles : j + 3 >= n_tiles)) return;
-            issue_one(n, S, (S + 3) & 3, j + 4, j + 3);
+            if constexpr (kMode == kPaged) {
+                dma_rows(is_k, is_k ? rows_k : rows_v, is_k ? S : (S + 3) & 3, is_k ? n : n - G::IPW);
+            } else {
+                issue_one(n, S, (S + 3) & 3, j + 4, j + 3);
+            }
         };
 
         // ---- A ----
@@ -483,7 +607,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             }
             dma(2, ks);
             if (ks == G::KS / 2) {
-                if (next_ok) lm0 = mask_max(s_out[0], 0, j + 1, next_masked);
+                if (next_ok) lm0 = mask_max(s_out[0], 0, j + 1, next_masked, next_holes);
             }
             Fence();
         }
@@ -496,7 +620,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             Fence();
             if constexpr (i == 1) {
                 asm volatile("s_nop 4");
-                if (next_ok) lm1 = mask_max(s_out[1], 1, j + 1, next_masked);
+                if (next_ok) lm1 = mask_max(s_out[1], 1, j + 1, next_masked, next_holes);
             }
             if constexpr (i >= 1) {
                 // KS K reads over the MFMAs 1 .. NPV-1 (kf was last read two MFMAs ago).
@@ -509,6 +633,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             dma(3, i);
             Fence();
         });
+        if constexpr (kMode == kPaged) rows_v = rows_k;
         // ---- rare rescale for tile j+1 ----
         if (next_ok) rescale_if_grown(lm0, lm1);
         Fence();
@@ -523,12 +648,35 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
     };
 
     int j = 0;
-    // Steady state: plain tiles with the full ring ahead, four steps per trip.
-    for (; j + 5 <= n_plain && j + 8 <= n_tiles; j += 4) {
+    // Steady state: plain tiles with the full ring ahead, four steps per trip. (Paged: without holes, too.
+    // The trip's page ids were asked for a trip ago.)
+    int ids[kMode == kPaged ? 8 : 1];
+    auto ask_ids = [&](int t) __attribute__((always_inline)) {
+        if constexpr (kMode == kPaged) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ids[i] = half_id(t + i / 2, i % 2);
+        }
+    };
+    auto no_holes = [&](int t) __attribute__((always_inline)) -> bool {
+        if constexpr (kMode == kPaged) {
+            int holes4 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) holes4 |= holes_of(t + i, ids[2 * i], ids[2 * i + 1]);
+            return holes4 == 0;
+        }
+        return true;
+    };
+    ask_ids(1);
+    for (; j + 5 <= n_plain && j + 8 <= n_tiles && no_holes(j + 1); j += 4) {
+        ask_ids(j + 5);
         step.template operator()<false, 0>(j, s0, s1);
         step.template operator()<false, 1>(j + 1, s1, s0);
         step.template operator()<false, 2>(j + 2, s0, s1);
         step.template operator()<false, 3>(j + 3, s1, s0);
+    }
+    if constexpr (kMode == kPaged) {
+        id_half0 = half_id(j + 1, 0);
+        id_half1 = half_id(j + 1, 1);
     }
     // Tail (j is a multiple of 4 here): masked steps, same slot rotation.
     for (; j < n_tiles; j += 4) {
@@ -588,7 +736,9 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
                 w0 *= c;
                 w1 *= c;
             }
-            const int64_t at = split * p.batch * p.num_heads * seq_q + flat;
+            const int64_t at = kMode == kPaged
+                                   ? job.state + static_cast<int64_t>(row) * pack + hl[R]
+                                   : split * p.batch * p.num_heads * seq_q + flat;
 #pragma unroll
             for (int dt = 0; dt < G::DT; ++dt) {
                 float a[16];
@@ -622,7 +772,13 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
             }
             StoreTile<M>(out_row + 32 * dt, hh, row_ok, a);
         }
-        if (row_ok && p.lse != nullptr && hh == 0) {
+        if constexpr (kMode == kPaged) {
+            if (row_ok && p.lse != nullptr && hh == 0) {
+                // (the bits: compiled without regard to NaN, a comparison could take a NaN sum for none)
+                const bool none = __builtin_bit_cast(uint32_t, l_lse) == 0;
+                p.lse[(tok_q + row) * p.num_heads + h] = none ? neg_inf() : (mm + __log2f(l_lse)) * kLn2;
+            }
+        } else if (row_ok && p.lse != nullptr && hh == 0) {
             p.lse[flat] = l_lse > 0.0f ? (mm + __log2f(l_lse)) * kLn2 : neg_inf();
         }
     };
@@ -637,6 +793,12 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel
     } else {
         finish.template operator()<1>();
     }
+}
+
+template <typename E, int D, bool kCausal, WideMode kMode, Denominator kDen>
+__global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void flash_fwd_wide_kernel(
+    const sca_flash_params p, int num_q_tiles, const VarlenArgs vl, const SplitArgs sp) {
+    FlashWide<E, D, kCausal, kMode, kDen>(p, num_q_tiles, vl, sp, PagedJob{});
 }
 
 }  // namespace

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <map>
 #include <string>
 #include <vector>
 
@@ -18,7 +19,7 @@ constexpr int kCombineThreads = 256;
 constexpr int64_t kMostScratch = int64_t{64} << 20;
 
 // out = sum_s O_s 2^(mu_s - mu*) / sum_s l_s 2^(mu_s - mu*), one thread per (row, 4 dims); grid.y is
-// the sequence. A range that saw no key has l = 0 and counts for nothing.
+// the sequence. A range that saw no key left zeros.
 template <typename E>
 __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(const PagedArgs p,
                                                                         const PagedSeqs seqs,
@@ -35,23 +36,46 @@ __global__ __launch_bounds__(kCombineThreads) void paged_combine_kernel(const Pa
     const uint32_t d0 = (idx - at * quads) * 4;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + sq.state_base + at;
     const float* po = p.part_o + (static_cast<int64_t>(sq.state_base) + at) * head_dim + d0;
+    // Up to sixteen states at a time, all requested before the first is used, so that a merge waits for
+    // memory once or twice: with four at a time, twice over for the maximum, 18 states of 160 rows took
+    // 12.8 us (6.2 so).
     float mu = neg_inf();
-#pragma unroll 4
-    for (int s = 0; s < sq.splits; ++s) mu = fmaxf(mu, ml[static_cast<int64_t>(s) * all].x);
     float l = 0.0f;
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < sq.splits; ++s) {
-        const float2 st = ml[static_cast<int64_t>(s) * all];
-        if (st.y == 0.0f) continue;
-        // (a range whose scores were all NaN has no maximum but a NaN sum, which must stay)
-        const float w = st.x == neg_inf() ? 1.0f : fast_exp2(st.x - mu);
-        l = fmaf(st.y, w, l);
-        const float4 v = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * all * head_dim);
-        a[0] = fmaf(v.x, w, a[0]);
-        a[1] = fmaf(v.y, w, a[1]);
-        a[2] = fmaf(v.z, w, a[2]);
-        a[3] = fmaf(v.w, w, a[3]);
+    auto merge = [&]<int kAtOnce>(int s0) __attribute__((always_inline)) {
+        float2 st[kAtOnce];
+        floatx4 v[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t s = min(s0 + i, sq.splits - 1);  // (repeats of the last one do not count)
+            st[i] = ml[s * all];
+            v[i] = *reinterpret_cast<const floatx4*>(po + s * all * head_dim);
+        }
+        float top = mu;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
+        const float back = mu == neg_inf() ? 1.0f : fast_exp2(mu - top);
+        l *= back;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) a[d] *= back;
+        mu = top;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            // (a state without a maximum is zeros, or NaN where its scores were, which must stay)
+            const float w = st[i].x == neg_inf() ? 1.0f : fast_exp2(st[i].x - mu);
+            if (s0 + i < sq.splits) {
+                l = fmaf(st[i].y, w, l);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) a[d] = fmaf(v[i][d], w, a[d]);
+            }
+        }
+    };
+    if (sq.splits == 2) {
+        merge.template operator()<2>(0);
+    } else if (sq.splits <= 4) {
+        merge.template operator()<4>(0);
+    } else {
+        for (int s0 = 0; s0 < sq.splits; s0 += 16) merge.template operator()<16>(s0);
     }
     const float inv = l > 0.0f ? 1.0f / l : l;
     const uint32_t h_kv = at / rows;
@@ -70,8 +94,8 @@ bool Aligned(const void* ptr, uintptr_t bytes) {
     return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0;
 }
 
-// The kernels that serve a call: tiles of 128 rows, or the few-token kernel's 16 or 32.
-enum Kind { kTile, kFew16, kFew32 };
+// The kernels that serve a call: tiles of 128 rows (wide or general), or the few-token kernel's 16 or 32.
+enum Kind { kWide, kTile, kFew16, kFew32 };
 
 struct Launch {
     Kind kind;
@@ -90,27 +114,92 @@ struct Plan {
 Kind KindFor(const sca_paged_varlen_params& p, int64_t rows) {
     if (rows <= 16) return kFew16;
     if (rows <= 32) return p.head_dim <= 192 ? kFew32 : kFew16;
-    return kTile;
+    // (the wide kernel addresses 16 rows of a page with 32-bit offsets)
+    const bool wide = p.k_exp == nullptr && p.head_dim <= 160 && p.block_size >= 16 && p.k_ss < (1 << 25) &&
+                      p.v_ss < (1 << 25);
+    return wide ? kWide : kTile;
 }
 
-int RowsPerTile(Kind kind) { return kind == kTile ? kPagedRows : kind == kFew32 ? 32 : 16; }
+bool IsFew(Kind kind) { return kind == kFew16 || kind == kFew32; }
+int RowsPerTile(Kind kind) { return !IsFew(kind) ? kPagedRows : kind == kFew32 ? 32 : 16; }
 
 // Keys that a workgroup takes in one step.
-int KeysPerStep(Kind kind, int64_t head_dim) { return kind != kTile ? 128 : head_dim <= 128 ? 64 : 32; }
+int KeysPerStep(Kind kind, int64_t head_dim) {
+    return IsFew(kind) ? 128 : kind == kWide || head_dim <= 128 ? 64 : 32;
+}
 
 // Workgroups that the GPU holds at once.
 int64_t Resident(Kind kind, const sca_paged_varlen_params& p) {
     const int d = static_cast<int>(p.head_dim);
-    const int on_cu = kind == kTile ? (d <= 128 ? 2 : 1) : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
+    const int on_cu = kind == kWide   ? (d <= 64 ? 2 : 1)
+                      : kind == kTile ? (d <= 128 ? 2 : 1)
+                                      : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
     return static_cast<int64_t>(CuCount()) * on_cu;
+}
+
+struct Entry {
+    PagedSeq seq;
+    int64_t steps;   // of its last row tile
+    int64_t steps0;  // of its first (the same without a causal mask)
+};
+
+// Splits that keep a unit to `span` steps, where that saves enough of them to be worth the states'
+// traffic.
+int32_t SplitsFor(Kind kind, int64_t steps, int64_t span) {
+    if (steps - span < (IsFew(kind) ? 3 : 8)) return 1;
+    return static_cast<int32_t>(std::min<int64_t>(64, (steps + span - 1) / span));
+}
+
+// Longest units first.
+void Order(std::vector<Entry>* list) {
+    std::stable_sort(list->begin(), list->end(), [](const Entry& a, const Entry& b) {
+        return a.steps * b.seq.splits > b.steps * a.seq.splits;
+    });
+}
+
+// Steps (about a microsecond each) until the last of the units ends, each given to the workgroup slot that
+// is free first; a sequence's row tiles in up to four groups of equal length. What a unit does besides its
+// steps counts as kOverhead of them, the merge as kMerge and the states' way through memory.
+constexpr size_t kSimulated = 32;
+int64_t Makespan(const std::vector<Entry>& list, const sca_paged_varlen_params& p, Kind kind, int64_t resident) {
+    const int64_t overhead = IsFew(kind) ? 2 : 6, merge = 5;
+    std::map<int64_t, int64_t> free_at;  // slots by the time they are free
+    free_at[0] = resident;
+    int64_t end = 0, states = 0;
+    for (const Entry& e : list) {
+        const int64_t groups = std::min<int64_t>(4, e.seq.row_tiles);
+        for (int64_t g = groups - 1; g >= 0; --g) {
+            const int64_t steps = e.steps0 + (e.steps - e.steps0) * (2 * g + 1) / (2 * groups);
+            int64_t units = (e.seq.row_tiles * (g + 1) / groups - e.seq.row_tiles * g / groups) * e.seq.splits *
+                            p.num_kv_heads;
+            const int64_t takes = (steps + e.seq.splits - 1) / e.seq.splits + overhead;
+            if (units > 16 * resident) {  // many rounds alike
+                const int64_t rounds = units / resident - 8;
+                std::map<int64_t, int64_t> later;
+                for (const auto& slot : free_at) later[slot.first + rounds * takes] = slot.second;
+                free_at.swap(later);
+                units -= rounds * resident;
+            }
+            while (units > 0) {
+                const auto first = free_at.begin();
+                const int64_t time = first->first, n = std::min(units, first->second);
+                if (n == first->second) {
+                    free_at.erase(first);
+                } else {
+                    first->second -= n;
+                }
+                free_at[time + takes] += n;
+                end = std::max(end, time + takes);
+                units -= n;
+            }
+        }
+        if (e.seq.splits > 1) states += static_cast<int64_t>(e.seq.q_count) * p.num_heads * e.seq.splits;
+    }
+    return states == 0 ? end : end + merge + states * (p.head_dim + 2) / 500000;
 }
 
 // The launches of one kind, appended to `plan`. States of split keys may go to `most_states` of scratch.
 void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, Plan* plan) {
-    struct Entry {
-        PagedSeq seq;
-        int64_t steps;  // of its last row tile
-    };
     const int64_t group = p.num_heads / p.num_kv_heads;
     const int64_t rows_per_tile = RowsPerTile(kind);
     const int64_t keys = KeysPerStep(kind, p.head_dim);
@@ -127,28 +216,34 @@ void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, 
         e.seq.splits = 1;
         e.seq.row_tiles = static_cast<int32_t>((n * group + rows_per_tile - 1) / rows_per_tile);
         e.steps = (p.kv_lens[s] + keys - 1) / keys;
-        // (causal: the row tiles of new tokens see fewer keys; their mean serves the estimate)
-        const int64_t mean =
-            p.causal ? std::max<int64_t>(1, e.steps - std::min<int64_t>(n, p.kv_lens[s]) / (2 * keys)) : e.steps;
-        work += p.num_kv_heads * e.seq.row_tiles * mean;
+        const int64_t seen = p.kv_lens[s] - n + std::min<int64_t>(n, (rows_per_tile + group - 1) / group);
+        e.steps0 = p.causal ? std::max<int64_t>(0, (seen + keys - 1) / keys) : e.steps;
+        work += p.num_kv_heads * e.seq.row_tiles * ((e.steps + e.steps0 + 1) / 2);
         list.push_back(e);
     }
     if (list.empty()) return;
-    // Key splits: every unit at most the share of one resident workgroup, for the sequences where that
-    // saves enough steps of the longest unit to pay for the states' traffic and the merge's launch (a
-    // step takes about 1 us in either kernel, those 5 us and more).
-    const int64_t least = kind == kTile ? 4 : 1, worth = kind == kTile ? 8 : 3;
     const int64_t resident = Resident(kind, p);
-    const int64_t span = std::max(least, (work + resident - 1) / resident);
-    for (Entry& e : list) {
-        if (most_states > 0 && e.steps - span >= worth) {
-            e.seq.splits = static_cast<int32_t>(std::min<int64_t>(64, (e.steps + span - 1) / span));
+    if (most_states > 0) {
+        const int64_t share = std::max<int64_t>(1, (work + resident - 1) / resident);
+        int64_t span = share;
+        if (list.size() <= kSimulated) {
+            // The span of keys per unit with the least estimated run, from half a workgroup's share of
+            // the work to all keys.
+            int64_t least = -1;
+            for (const int quarters : {2, 3, 4, 5, 6, 8, 12, 1 << 20}) {
+                const int64_t tried = std::max<int64_t>(IsFew(kind) ? 1 : 4, share * quarters / 4);
+                for (Entry& e : list) e.seq.splits = SplitsFor(kind, e.steps, tried);
+                Order(&list);
+                const int64_t run = Makespan(list, p, kind, resident);
+                if (least < 0 || run < least) {
+                    least = run;
+                    span = tried;
+                }
+            }
         }
+        for (Entry& e : list) e.seq.splits = SplitsFor(kind, e.steps, span);
     }
-    // Longest units first.
-    std::stable_sort(list.begin(), list.end(), [](const Entry& a, const Entry& b) {
-        return a.steps * b.seq.splits > b.steps * a.seq.splits;
-    });
+    Order(&list);
     for (size_t at = 0; at < list.size(); at += kPagedSeqs) {
         Launch launch{};
         launch.kind = kind;
@@ -174,7 +269,7 @@ void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, 
 // Long chunks first: the few-token launches fill the GPU behind them.
 Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
     Plan plan;
-    for (Kind kind : {kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
+    for (Kind kind : {kWide, kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
     return plan;
 }
 
@@ -184,6 +279,9 @@ template <typename E, int D, bool kHeld8>
 int LaunchKind(const PagedArgs& a, const Launch& l, hipStream_t s) {
     const int units = static_cast<int>(l.units);
     if (l.kind == kTile) return LaunchPagedTile<E, D, kHeld8>(a, l.seqs, units, s);
+    if constexpr (!kHeld8 && D <= 160) {
+        if (l.kind == kWide) return LaunchPagedWide<E, D>(a, l.seqs, units, s);
+    }
     if constexpr (D <= 192) {
         if (l.kind == kFew32) return LaunchPagedFew<E, D, kHeld8, 2>(a, l.seqs, units, s);
     }

@@ -69,6 +69,8 @@ static_assert(sizeof(PagedArgs) + sizeof(PagedSeqs) <= 4096, "kernel arguments")
 // Launchers, instantiated in the file of their kernel; `units` workgroups.
 template <typename E, int D, bool kHeld8>
 int LaunchPagedTile(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_tile.hpp
+template <typename E, int D>
+int LaunchPagedWide(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_wide.hpp
 template <typename E, int D, bool kHeld8, int NC>
 int LaunchPagedFew(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_few.hpp
 
