@@ -49,7 +49,8 @@ HIP_FLAGS = [
 # (Not flash_fwd.hip: its merge of key splits tells an empty state from a NaN one.)
 FILE_FLAGS = {name: ["-fno-honor-nans"] for name in
               ("flash_reg.hip", "flash_pair.hip", "flash_wide_fp16.hip",
-               "flash_wide_bf16.hip", "flash_dsplit.hip", "paged_wide_fp16.hip", "paged_wide_bf16.hip")}
+               "flash_wide_bf16.hip", "flash_dsplit.hip", "paged_wide_fp16.hip", "paged_wide_bf16.hip",
+               "paged_dsplit.hip")}
 
 HOST_FLAGS = [
     "-std=c++20",

@@ -179,7 +179,75 @@ int LaunchFlashDsplit(const sca_flash_params& p, const SplitArgs& sp, hipStream_
 template <typename E, int D, bool kCausal>
 int LaunchFlashVarlen(const sca_flash_varlen_params& v, hipStream_t s);  // flash_wide.hpp
 
+// A workgroup's share of a launch over paged KV: packed rows of one row tile and KV head, and
+// a range of key tiles. Pages of at least 16 tokens.
+struct PagedJob {
+    const int32_t* table;   // the sequence's row of the page table
+    int64_t max_blocks, num_blocks;
+    int block_shift;
+    int q_first, q_count, keys;
+    int tile, split, splits, h_kv;
+    int64_t state;          // splits > 1: the state of packed row 0 of this (split, KV head)
+};
+
 namespace {
+
+// Where the keys of a PagedJob lie. Page ids come through the scalar cache (their addresses are uniform
+// per wave); everything is without branches and in 32 bits (keys and pool rows are below 2^31).
+struct PagedKeys {
+    const __attribute__((address_space(4))) int32_t* table;
+    uint32_t num_blocks;
+    int shift;
+    int mapped;     // keys that the table's row covers
+    int last_page;  // the last entry that is read
+
+    __device__ __forceinline__ explicit PagedKeys(const PagedJob& job)
+        : table((const __attribute__((address_space(4))) int32_t*)(job.table)),
+          num_blocks(static_cast<uint32_t>(job.num_blocks)),
+          shift(job.block_shift),
+          mapped(static_cast<int>(min(static_cast<int64_t>(job.keys), job.max_blocks << job.block_shift))),
+          last_page(max(0, mapped - 1) >> job.block_shift) {}
+
+    __device__ __forceinline__ int id(int key) const { return table[min(key >> shift, last_page)]; }
+    __device__ __forceinline__ bool in_pool(int id) const {
+        return static_cast<uint32_t>(id) < num_blocks;  // (negative ids are large ones)
+    }
+    // Key `key`'s page `id` does not hold it.
+    __device__ __forceinline__ bool hole(int key, int id) const { return !in_pool(id) | (key >= mapped); }
+};
+
+// The first key of [key, end) that lies on a page that is not mapped, or end: one look at the ids of a
+// range's pages, 512 at a time, so that the tiles before need none. The same on every lane.
+__device__ __forceinline__ int FirstHole(const PagedKeys& k, const int32_t* table, int key, int end) {
+    const int stop = min(end, k.mapped);
+    if (key >= stop) return min(key, end);
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    const int last = (stop - 1) >> k.shift;
+    for (int page = key >> k.shift; page <= last; page += 8 * kWave) {
+        int ids[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ids[i] = table[min(page + i * kWave + lane, last)];
+        int bad = -1;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const uint64_t out = __builtin_amdgcn_ballot_w64(!k.in_pool(ids[i]));
+            bad = out != 0 ? page + i * kWave + __builtin_ctzll(out) : bad;
+        }
+        if (bad >= 0) return max(key, bad << k.shift);
+    }
+    return stop;
+}
+
+// Up to `most` pool rows of one page, from key `key` on page `id` to key `end`.
+struct PagedRows {
+    uint32_t row;
+    int count;  // 0 or less: none
+};
+__device__ __forceinline__ PagedRows RowsAt(const PagedKeys& k, int key, int id, int most, int end) {
+    const bool ok = k.in_pool(id);
+    const uint32_t row = (static_cast<uint32_t>(id) << k.shift) + (static_cast<uint32_t>(key) & ((1u << k.shift) - 1));
+    return {ok ? row : 0, ok ? min(most, min(k.mapped, end) - key) : 0};
+}
 
 template <typename E>
 struct Mfma;
@@ -476,6 +544,15 @@ __device__ __forceinline__ void DmaToLds(const uint8_t* base, int num_records, u
         const_cast<uint8_t*>(base), 0, num_records, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds), 16,
                                              voffset, soffset, 0, 0);
+}
+
+// The same from rows of a page: a buffer resource of its own, bounded at the rows that exist, makes the
+// others read as zeros (keys past the end, pages that are not mapped).
+template <int ROW_BYTES>
+__device__ __forceinline__ void DmaRowsToLds(const uint8_t* base, int row_bytes, const PagedRows& r,
+                                             uint8_t* lds, uint32_t voffset) {
+    const uint8_t* at = base + static_cast<uint64_t>(r.row) * static_cast<uint32_t>(row_bytes);
+    DmaToLds(at, r.count > 0 ? (r.count - 1) * row_bytes + ROW_BYTES : 0, lds, voffset, 0);
 }
 
 // MFMAs issued from inline asm: S^T accumulators in VGPRs, O^T accumulators in AGPRs.

@@ -94,8 +94,9 @@ bool Aligned(const void* ptr, uintptr_t bytes) {
     return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0;
 }
 
-// The kernels that serve a call: tiles of 128 rows (wide or general), or the few-token kernel's 16 or 32.
-enum Kind { kWide, kTile, kFew16, kFew32 };
+// The kernels that serve a call: tiles of 128 rows (the flash kernels over pages, or the general one), or
+// the few-token kernel's 16 or 32.
+enum Kind { kFlash, kTile, kFew16, kFew32 };
 
 struct Launch {
     Kind kind;
@@ -114,10 +115,9 @@ struct Plan {
 Kind KindFor(const sca_paged_varlen_params& p, int64_t rows) {
     if (rows <= 16) return kFew16;
     if (rows <= 32) return p.head_dim <= 192 ? kFew32 : kFew16;
-    // (the wide kernel addresses 16 rows of a page with 32-bit offsets)
-    const bool wide = p.k_exp == nullptr && p.head_dim <= 160 && p.block_size >= 16 && p.k_ss < (1 << 25) &&
-                      p.v_ss < (1 << 25);
-    return wide ? kWide : kTile;
+    // (the flash kernels address 16 rows of a page with 32-bit offsets)
+    const bool flash = p.k_exp == nullptr && p.block_size >= 16 && p.k_ss < (1 << 25) && p.v_ss < (1 << 25);
+    return flash ? kFlash : kTile;
 }
 
 bool IsFew(Kind kind) { return kind == kFew16 || kind == kFew32; }
@@ -125,13 +125,13 @@ int RowsPerTile(Kind kind) { return !IsFew(kind) ? kPagedRows : kind == kFew32 ?
 
 // Keys that a workgroup takes in one step.
 int KeysPerStep(Kind kind, int64_t head_dim) {
-    return IsFew(kind) ? 128 : kind == kWide || head_dim <= 128 ? 64 : 32;
+    return IsFew(kind) ? 128 : head_dim <= (kind == kFlash ? 160 : 128) ? 64 : 32;
 }
 
 // Workgroups that the GPU holds at once.
 int64_t Resident(Kind kind, const sca_paged_varlen_params& p) {
     const int d = static_cast<int>(p.head_dim);
-    const int on_cu = kind == kWide   ? (d <= 64 ? 2 : 1)
+    const int on_cu = kind == kFlash   ? (d <= 64 ? 2 : 1)
                       : kind == kTile ? (d <= 128 ? 2 : 1)
                                       : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
     return static_cast<int64_t>(CuCount()) * on_cu;
@@ -269,7 +269,7 @@ void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, 
 // Long chunks first: the few-token launches fill the GPU behind them.
 Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
     Plan plan;
-    for (Kind kind : {kWide, kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
+    for (Kind kind : {kFlash, kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
     return plan;
 }
 
@@ -279,8 +279,11 @@ template <typename E, int D, bool kHeld8>
 int LaunchKind(const PagedArgs& a, const Launch& l, hipStream_t s) {
     const int units = static_cast<int>(l.units);
     if (l.kind == kTile) return LaunchPagedTile<E, D, kHeld8>(a, l.seqs, units, s);
-    if constexpr (!kHeld8 && D <= 160) {
-        if (l.kind == kWide) return LaunchPagedWide<E, D>(a, l.seqs, units, s);
+    if constexpr (!kHeld8) {
+        if (l.kind == kFlash) {
+            if constexpr (D <= 160) return LaunchPagedWide<E, D>(a, l.seqs, units, s);
+            else return LaunchPagedDsplit<E, D>(a, l.seqs, units, s);
+        }
     }
     if constexpr (D <= 192) {
         if (l.kind == kFew32) return LaunchPagedFew<E, D, kHeld8, 2>(a, l.seqs, units, s);

@@ -71,6 +71,8 @@ template <typename E, int D, bool kHeld8>
 int LaunchPagedTile(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_tile.hpp
 template <typename E, int D>
 int LaunchPagedWide(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_wide.hpp
+template <typename E, int D>
+int LaunchPagedDsplit(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_dsplit.hip
 template <typename E, int D, bool kHeld8, int NC>
 int LaunchPagedFew(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_few.hpp
 

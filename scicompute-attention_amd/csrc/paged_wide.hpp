@@ -7,7 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include "flash_wide.hpp"
-#include "paged_varlen.hpp"
+#include "paged_job.hpp"
 
 namespace sca_hip {
 namespace {
@@ -16,29 +16,15 @@ template <typename E, int D, Denominator kDen>
 __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void paged_wide_kernel(const PagedArgs a,
                                                                              const PagedSeqs seqs) {
     static_assert(WideGeom<D>::BM == kPagedRows);
-    const PagedUnit u = FindUnit(seqs, a.kv_heads);
-    const PagedSeq& sq = u.seq;
-    sca_flash_params p{};
-    p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out, p.lse = a.lse;
-    p.batch = 1;
-    p.num_heads = a.heads;
-    p.num_kv_heads = a.kv_heads;
-    p.q_sh = a.q_sh, p.q_ss = a.q_ss;
-    p.k_sh = a.k_sh, p.k_ss = a.k_ss;
-    p.v_sh = a.v_sh, p.v_ss = a.v_ss;
-    p.o_sh = a.o_sh, p.o_ss = a.o_ss;
-    p.scale = a.scale;
-    // Without a causal mask the diagonal lies behind the last key.
-    p.diagonal = a.causal ? sq.keys - sq.q_count : sq.keys;
-    PagedJob job{};
-    job.table = a.page_table + static_cast<int64_t>(sq.table_row) * a.max_blocks;
-    job.max_blocks = a.max_blocks, job.num_blocks = a.num_blocks;
-    job.block_shift = a.block_shift;
-    job.q_first = sq.q_first, job.q_count = sq.q_count, job.keys = sq.keys;
-    job.tile = u.tile, job.split = u.split, job.splits = sq.splits, job.h_kv = u.h_kv;
-    job.state = sq.state_base + (static_cast<int64_t>(u.split) * a.kv_heads + u.h_kv) * sq.q_count * a.group;
-    FlashWide<E, D, true, kPaged, kDen>(p, 0, VarlenArgs{nullptr, nullptr, nullptr},
-                                        SplitArgs{a.group, 1, a.part_o, a.part_ml}, job);
+    sca_flash_params p;
+    PagedJob job;
+    JobOf(a, seqs, &p, &job);
+    const SplitArgs sp{a.group, 1, a.part_o, a.part_ml};
+    const VarlenArgs vl{nullptr, nullptr, nullptr};
+    constexpr bool kCausal = true;
+    constexpr WideMode kMode = kPaged;
+    constexpr int num_q_tiles = 0;
+#include "flash_wide_body.hpp"
 }
 
 }  // namespace
