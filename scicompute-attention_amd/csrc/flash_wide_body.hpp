@@ -598,6 +598,16 @@
     }
 
     // ---- epilogue: merge the key halves of each row group, normalise, store ----
+    if constexpr (kMode == kPaged) {
+        // Heads once more (pinned, or they would be held over the loop: at D 64 the registers decide whether
+        // a CU holds two workgroups).
+#pragma unroll
+        for (int r = 0; r < G::RT; ++r) {
+            int row = q0 + 64 * rg + 32 * r + lr;
+            asm volatile("" : "+v"(row));
+            hl[r] = row - qi[r] * pack;
+        }
+    }
     WaitVm<0>();
     SettleO(o);
     __builtin_amdgcn_s_barrier();

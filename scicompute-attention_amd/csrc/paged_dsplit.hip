@@ -23,7 +23,7 @@ __global__ __launch_bounds__(DsplitGeom<D>::THREADS, 1) void paged_dsplit_kernel
     static_assert(DsplitGeom<D>::BM == kPagedRows);
     sca_flash_params p;
     PagedJob job;
-    JobOf(a, seqs, &p, &job);
+    JobOf(a, FindUnit(seqs, a.kv_heads, static_cast<int>(blockIdx.x)), &p, &job);
     const SplitArgs sp{a.group, 1, a.part_o, a.part_ml};
     constexpr bool kCausal = true, kCut = true, kPaged = true;
     constexpr int num_q_tiles = 0;

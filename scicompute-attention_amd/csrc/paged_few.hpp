@@ -35,6 +35,7 @@ struct FewGeom {
     static constexpr int CPR = kHeld8 ? D / 16 : D / 8;   // 16-byte chunks of a row in memory
     static constexpr int NV = kMfmaTile * CPR / kWave;    // V loads per lane and tile
     static constexpr int TILE_BYTES = kMfmaTile * RB;
+    static constexpr int V_BYTES = kDecodeWaves * TILE_BYTES;
     // Registers: O and Q of NC groups, a tile's K and V.
     static constexpr int WAVES = FewResident(D, kHeld8, NC);
 };
@@ -50,23 +51,19 @@ struct FewMfma<BF16> {
     using M = DecMfma<DecBF16>;
 };
 
+// A unit's work, with LDS for the waves' V tiles and for (m, l).
 template <typename E, int D, bool kHeld8, int NC>
-__global__ __launch_bounds__(kDecodeThreads, (FewGeom<D, kHeld8, NC>::WAVES)) void paged_few_kernel(
-    const PagedArgs p, const PagedSeqs seqs) {
+__device__ __forceinline__ void FewUnit(const PagedArgs& p, const PagedUnit& u, uint8_t* s_v,
+                                        float (*s_m)[16 * NC], float (*s_l)[16 * NC]) {
     using G = FewGeom<D, kHeld8, NC>;
     using M = typename FewMfma<E>::M;
     using vec8 = typename M::vec8;
-
-    __shared__ __align__(16) uint8_t s_v[kDecodeWaves * G::TILE_BYTES];
-    __shared__ float s_m[kDecodeWaves][G::ROWS];
-    __shared__ float s_l[kDecodeWaves][G::ROWS];
 
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane % 16;
     const int grp = lane / 16;
 
-    const PagedUnit u = FindUnit(seqs, p.kv_heads);
     const PagedSeq& sq = u.seq;
     const int rows = sq.q_count * p.group;
     const int diag = p.causal ? sq.keys - sq.q_count : 0;
@@ -344,10 +341,20 @@ __global__ __launch_bounds__(kDecodeThreads, (FewGeom<D, kHeld8, NC>::WAVES)) vo
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out_row * p.o_ss + head * p.o_sh + d) =
                 make_uint2(M::pack(osum[0] * inv, osum[1] * inv), M::pack(osum[2] * inv, osum[3] * inv));
             if (p.lse != nullptr && d == 0) {
-                p.lse[out_row * p.heads + head] = lsum == 0.0f ? neg_inf() : (mm + __log2f(lsum)) * kLn2;
+                p.lse[out_row * p.heads + head] = __builtin_bit_cast(uint32_t, lsum) == 0 ? neg_inf() : (mm + __log2f(lsum)) * kLn2;
             }
         }
     }
+}
+
+template <typename E, int D, bool kHeld8, int NC>
+__global__ __launch_bounds__(kDecodeThreads, (FewGeom<D, kHeld8, NC>::WAVES)) void paged_few_kernel(
+    const PagedArgs p, const PagedSeqs seqs) {
+    using G = FewGeom<D, kHeld8, NC>;
+    __shared__ __align__(16) uint8_t s_v[G::V_BYTES];
+    __shared__ float s_m[kDecodeWaves][G::ROWS];
+    __shared__ float s_l[kDecodeWaves][G::ROWS];
+    FewUnit<E, D, kHeld8, NC>(p, FindUnit(seqs, p.kv_heads, static_cast<int>(blockIdx.x)), s_v, s_m, s_l);
 }
 
 }  // namespace

@@ -8,9 +8,7 @@
 namespace sca_hip {
 namespace {
 
-__device__ __forceinline__ void JobOf(const PagedArgs& a, const PagedSeqs& seqs, sca_flash_params* p,
-                                      PagedJob* job) {
-    const PagedUnit u = FindUnit(seqs, a.kv_heads);
+__device__ __forceinline__ void JobOf(const PagedArgs& a, const PagedUnit& u, sca_flash_params* p, PagedJob* job) {
     const PagedSeq& sq = u.seq;
     *p = sca_flash_params{};
     p->q = a.q, p->k = a.k, p->v = a.v, p->out = a.out, p->lse = a.lse;

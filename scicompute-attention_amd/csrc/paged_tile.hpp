@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     const int lr = lane & 31;
     const int hh = lane >> 5;
 
-    const PagedUnit u = FindUnit(seqs, p.kv_heads);
+    const PagedUnit u = FindUnit(seqs, p.kv_heads, static_cast<int>(blockIdx.x));
     const PagedSeq& sq = u.seq;
     const int rows = sq.q_count * p.group;
     const int diag = p.causal ? sq.keys - sq.q_count : 0;

@@ -1,6 +1,6 @@
 // Attention of ragged chunks of new tokens over paged KV: the plan of a call (units, key splits, the
 // launches' sequence lists), the merge of key splits, the checks and the C entry points. The kernels
-// are in paged_tile.hpp and paged_few.hpp; paged_varlen.hpp describes rows, units and splits.
+// are in paged_wide.hpp, paged_dsplit.hip, paged_tile.hpp, paged_few.hpp and paged_mixed.hpp; paged_varlen.hpp describes rows, units and splits.
 
 #include <hip/hip_runtime.h>
 
@@ -96,13 +96,14 @@ bool Aligned(const void* ptr, uintptr_t bytes) {
 
 // The kernels that serve a call: tiles of 128 rows (the flash kernels over pages, or the general one), or
 // the few-token kernel's 16 or 32.
-enum Kind { kFlash, kTile, kFew16, kFew32 };
+enum Kind { kFlash, kTile, kFew16, kFew32, kMixed };
 
 struct Launch {
     Kind kind;
     PagedSeqs seqs;
     int64_t units;
     int64_t combine_rows;  // most (KV head, row) pairs of a split sequence; 0: no merge
+    int64_t states;        // that it leaves
 };
 
 struct Plan {
@@ -261,15 +262,43 @@ void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, 
             q.unit_end = static_cast<int32_t>(launch.units);  // (Validate bounds the units)
             launch.seqs.seq[launch.seqs.count++] = q;
         }
+        launch.states = states;
         plan->states = std::max(plan->states, states);
         plan->launches.push_back(launch);
     }
+}
+
+// Joins a launch of long chunks and one of single tokens (paged_mixed.hpp).
+void Mix(int64_t most_states, Plan* plan) {
+    auto& all = plan->launches;
+    auto is = [](Kind kind) { return [kind](const Launch& l) { return l.kind == kind; }; };
+    const auto flash = std::find_if(all.begin(), all.end(), is(kFlash));
+    const auto few = std::find_if(all.begin(), all.end(), is(kFew16));
+    if (flash == all.end() || few == all.end()) return;
+    const int64_t states = flash->states + few->states;
+    if (flash->seqs.count + few->seqs.count > kPagedSeqs || states > most_states) return;
+    Launch both = *few;
+    both.kind = kMixed;
+    both.seqs.few_units = static_cast<int32_t>(few->units);
+    for (int i = 0; i < flash->seqs.count; ++i) {
+        PagedSeq q = flash->seqs.seq[i];
+        q.unit_end += both.seqs.few_units;
+        q.state_base += static_cast<int32_t>(few->states);
+        both.seqs.seq[both.seqs.count++] = q;
+    }
+    both.units += flash->units;
+    both.states = states;
+    both.combine_rows = std::max(both.combine_rows, flash->combine_rows);
+    plan->states = std::max(plan->states, states);
+    *flash = both;
+    all.erase(few);
 }
 
 // Long chunks first: the few-token launches fill the GPU behind them.
 Plan MakePlan(const sca_paged_varlen_params& p, int64_t most_states) {
     Plan plan;
     for (Kind kind : {kFlash, kTile, kFew32, kFew16}) PlanKind(p, kind, most_states, &plan);
+    if (p.head_dim <= 64) Mix(most_states, &plan);
     return plan;
 }
 
@@ -280,6 +309,9 @@ int LaunchKind(const PagedArgs& a, const Launch& l, hipStream_t s) {
     const int units = static_cast<int>(l.units);
     if (l.kind == kTile) return LaunchPagedTile<E, D, kHeld8>(a, l.seqs, units, s);
     if constexpr (!kHeld8) {
+        if constexpr (D <= 64) {
+            if (l.kind == kMixed) return LaunchPagedMixed<E, D>(a, l.seqs, units, s);
+        }
         if (l.kind == kFlash) {
             if constexpr (D <= 160) return LaunchPagedWide<E, D>(a, l.seqs, units, s);
             else return LaunchPagedDsplit<E, D>(a, l.seqs, units, s);

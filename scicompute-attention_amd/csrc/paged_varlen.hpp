@@ -44,7 +44,7 @@ struct PagedSeq {
 
 struct PagedSeqs {
     int32_t count;
-    int32_t reserved;
+    int32_t few_units;  // of the few-token kernel, ahead of the others (paged_mixed.hpp)
     PagedSeq seq[kPagedSeqs];
 };
 
@@ -73,19 +73,20 @@ template <typename E, int D>
 int LaunchPagedWide(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_wide.hpp
 template <typename E, int D>
 int LaunchPagedDsplit(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_dsplit.hip
+template <typename E, int D>
+int LaunchPagedMixed(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_mixed.hpp
 template <typename E, int D, bool kHeld8, int NC>
 int LaunchPagedFew(const PagedArgs& a, const PagedSeqs& seqs, int units, hipStream_t s);  // paged_few.hpp
 
 namespace {
 
-// The unit of this workgroup.
+// Unit w of a launch.
 struct PagedUnit {
     PagedSeq seq;
     int tile, split, h_kv;
 };
 
-__device__ __forceinline__ PagedUnit FindUnit(const PagedSeqs& seqs, int kv_heads) {
-    const int w = static_cast<int>(blockIdx.x);
+__device__ __forceinline__ PagedUnit FindUnit(const PagedSeqs& seqs, int kv_heads, int w) {
     int at = 0;
     if (seqs.count > 1) {
         // Sequences that end at or before unit w: every lane looks at two of them.

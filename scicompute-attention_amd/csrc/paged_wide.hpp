@@ -18,7 +18,7 @@ __global__ __launch_bounds__(WideGeom<D>::THREADS, 1) void paged_wide_kernel(con
     static_assert(WideGeom<D>::BM == kPagedRows);
     sca_flash_params p;
     PagedJob job;
-    JobOf(a, seqs, &p, &job);
+    JobOf(a, FindUnit(seqs, a.kv_heads, static_cast<int>(blockIdx.x)), &p, &job);
     const SplitArgs sp{a.group, 1, a.part_o, a.part_ml};
     const VarlenArgs vl{nullptr, nullptr, nullptr};
     constexpr bool kCausal = true;

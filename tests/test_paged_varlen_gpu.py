@@ -234,6 +234,46 @@ def test_large_scores_and_growing_maxima(hip, dtype, held8):
         check_lse(gl, lse, err, "ramp")
 
 
+@pytest.mark.parametrize("D", [32, 64, 128, 160, 192, 256])
+def test_unmapped_pages_under_long_chunks(hip, D):
+    """Holes at the first page, inside the steady part of the key loop, next to its end, and behind the first
+    512 pages; with and without split keys."""
+    for n, (L, holes) in enumerate([(400, (0,)), (1500, (0, 1, 17, 18, 50)), (1500, (93,)), (1500, (84,)), (9000, (540,))]):
+        def mutate(pl):
+            for i, h in enumerate(holes):
+                pl["table"][0, h] = -1 if i % 2 == 0 else pl["nb"]
+        case([L], [90], 16, 2, 2, D, "f16" if n % 2 else "bf16", False, 3300 + n, mutate=mutate)
+        case([L], [90], 16, 1, 1, D, "bf16", False, 3320 + n, mutate=mutate, scratches=(True,), causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [32, 64, 96])
+def test_chunks_and_single_tokens_in_one_step(hip, D, dtype):
+    lens = [2600, 1, 0, 3100, 700, 64, 1800, 5000, 65]
+    new = [300, 1, 0, 1, 40, 64, 1, 2, 1]
+    used = case(lens, new, 16, 8, 2, D, dtype, False, 3400 + D)
+    assert used > 0
+    case(lens, new, 16, 8, 2, D, dtype, False, 3400 + D, scratches=(used // 2, 4096))
+    case(lens, new, 32, 3, 1, D, dtype, False, 3410 + D, causal=False)
+    case([900, 900], [1, 200], 16, 16, 1, D, dtype, False, 3420 + D, first=2)
+
+
+@pytest.mark.parametrize("D", [32, 64])
+def test_nan_keys_of_a_single_token_beside_a_chunk(hip, D):
+    pl = pool([600, 600, 50], 16, 2, D, "bf16", 3500, False)
+    pl["k"][pl["table"][0, 10], 4, 1, 0] = 0x7FC0
+    pl["v"][pl["table"][1, 0], 0, 0, 3] = 0x7FC0
+    new, Hq = [1, 600, 1], 4
+    qb, _ = quantize(np.random.default_rng(3501).standard_normal((602, Hq, D)).astype(np.float32), "bf16")
+    for scratch in (0, True):
+        out, lse, _ = run(pl, new, qb, Hq, True, scratch)
+        want = np.zeros((602, Hq, D), bool)
+        want[0, 2:] = True          # a key: every dim of the heads that read it
+        want[1:601, :2, 3] = True   # a value: its own dim
+        assert np.array_equal(np.isnan(out), want)
+        assert np.array_equal(np.isnan(lse), want.all(axis=2))
+
+
 def test_strides_offsets_rows_of_the_table_and_repeated_sequences(hip):
     case([300, 20, 100], [4, 30, 2], 16, 4, 2, 64, "f16", False, 3000, first=3, rows=[0, 2, 0],
          use_lens=[300, 100, 250])
