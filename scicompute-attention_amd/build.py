@@ -50,7 +50,8 @@ HIP_FLAGS = [
 FILE_FLAGS = {name: ["-fno-honor-nans"] for name in
               ("flash_reg.hip", "flash_pair.hip", "flash_wide_fp16.hip",
                "flash_wide_bf16.hip", "flash_dsplit.hip", "paged_wide_fp16.hip", "paged_wide_bf16.hip",
-               "paged_dsplit.hip", "paged_mixed_fp16.hip", "paged_mixed_bf16.hip")}
+               "paged_dsplit.hip", "paged_mixed_fp16.hip", "paged_mixed_bf16.hip",
+               "paged_tile_fp16.hip", "paged_tile_bf16.hip")}
 
 HOST_FLAGS = [
     "-std=c++20",

@@ -1,12 +1,18 @@
-// The general kernel of attention over paged KV (paged_varlen.hpp): every head_dim, 16-bit and 8-bit
-// pages.
+// The general kernel of attention over paged KV (paged_varlen.hpp): 8-bit pages, pages of fewer than 16
+// tokens, and rows of pages more than 2^25 elements apart. The matrix units bound it.
 //
 // Four waves of 32 packed rows; key tiles of 64 keys (32 from head_dim 160 on) come through registers
 // into two LDS buffers: while a tile is multiplied the next one's loads are in flight, and 8-bit codes
-// are widened (e4m3.hpp) on their way into LDS, so that one inner loop serves both kinds of pages. A
-// lane looks up the page of one key per tile, one tile ahead of the loads that need it, and hands the
-// row to the lanes that copy it with a shuffle. Formulation, swizzles and online softmax are those of
-// the flash kernels (flash_common.hpp).
+// are widened (e4m3.hpp) on their way into LDS, once per workgroup, so that one inner loop serves both
+// kinds of pages. A lane looks up the page of one key per tile, one tile ahead of the loads that need it,
+// and hands the row to the lanes that copy it with a shuffle. Formulation, swizzles and online softmax are
+// those of the flash kernels (flash_common.hpp). Two workgroups to a CU up to D 128, so that one's
+// vector work runs beside the other's products.
+//
+// Measured (MI355X): 4 chunks of 2048 tokens behind 6,000 to 14,000, 8-bit pages, 32/8 heads, D 128: 1,735
+// us (924 TF/s; the wide kernel over 16-bit pages of the same content 1,657). Vector instructions per MFMA
+// decide: 10.3 before pool rows were multiplied in 32 bits, whole tiles left unmasked and maxima taken
+// without regard to NaN, 1,880 us. A higher wave priority over the products changes nothing.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -34,8 +40,6 @@ struct TileGeom {
 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (a plain vector stays in registers)
-
-__device__ __forceinline__ u32x4 Masked(const u32x4& w, uint32_t keep) { return w & keep; }
 
 // log2 headroom of the weights: they are 2^(x - mu) with mu that much below the row's maximum. fp16
 // weights then keep all their bits down to 2^-21 of the largest (2^-14 without), and stay finite: at
@@ -103,19 +107,20 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     constexpr int kEb = kHeld8 ? 1 : 2;
     const uint8_t* k_base = static_cast<const uint8_t*>(p.k) + u.h_kv * p.k_sh * kEb;
     const uint8_t* v_base = static_cast<const uint8_t*>(p.v) + u.h_kv * p.v_sh * kEb;
-    const int64_t k_row_bytes = p.k_ss * kEb;
-    const int64_t v_row_bytes = p.v_ss * kEb;
+    const uint32_t k_row_bytes = static_cast<uint32_t>(p.k_ss) * kEb, v_row_bytes = static_cast<uint32_t>(p.v_ss) * kEb;
     const int32_t* table = p.page_table + static_cast<int64_t>(sq.table_row) * p.max_blocks;
-    const int bs_mask = (1 << p.block_shift) - 1;
+    const uint32_t bs_mask = (1u << p.block_shift) - 1;
+    const uint32_t max_blocks = static_cast<uint32_t>(min(p.max_blocks, int64_t{0x7fffffff}));
+    const uint32_t num_blocks = static_cast<uint32_t>(p.num_blocks);
+    const int end = min(sq.keys, (first + n_tiles) * BN);
 
     // Pool row of key lane % BN of tile t, or -1 (past the keys, unmapped, outside the pool).
     auto row_of = [&](int t) __attribute__((always_inline)) -> int {
         const int key = t * BN + lane % BN;
-        const int logical = key >> p.block_shift;
-        if (t >= first + n_tiles || key >= sq.keys || logical >= p.max_blocks) return -1;
-        const int32_t id = table[logical];
-        if (id < 0 || id >= p.num_blocks) return -1;
-        return (id << p.block_shift) | (key & bs_mask);
+        const uint32_t logical = static_cast<uint32_t>(key) >> p.block_shift;
+        if (key >= end || logical >= max_blocks) return -1;
+        const uint32_t id = static_cast<uint32_t>(table[logical]);  // (negative ids are large ones)
+        return id < num_blocks ? static_cast<int>((id << p.block_shift) | (static_cast<uint32_t>(key) & bs_mask)) : -1;
     };
     u32x4 kr[G::PER], vr[G::PER];
     uint32_t k_byte = 0, v_byte = 0;  // exponent bytes of key lane % BN
@@ -124,8 +129,9 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
         valid = __builtin_amdgcn_ballot_w64(pool_row >= 0);
         const int safe = pool_row < 0 ? 0 : pool_row;
         if constexpr (kHeld8) {
-            const int64_t at = ((static_cast<int64_t>(safe >> p.block_shift) * p.kv_heads + u.h_kv)
-                                << p.block_shift) + (safe & bs_mask);
+            const uint32_t at_row = static_cast<uint32_t>(safe);
+            const uint64_t at = ((static_cast<uint64_t>(at_row >> p.block_shift) * static_cast<uint32_t>(p.kv_heads) +
+                                  static_cast<uint32_t>(u.h_kv)) << p.block_shift) + (at_row & bs_mask);
             k_byte = p.k_exp[at];
             v_byte = p.v_exp[at];
         }
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
         for (int i = 0; i < G::PER; ++i) {
             const int c = i * 256 + tid;
             if (G::CHUNKS % 256 != 0 && c >= G::CHUNKS) continue;
-            const int64_t r = __shfl(safe, c / G::CPR);
+            const uint64_t r = static_cast<uint32_t>(__shfl(safe, c / G::CPR));
             kr[i] = *reinterpret_cast<const u32x4*>(k_base + r * k_row_bytes + (c % G::CPR) * 16);
             vr[i] = *reinterpret_cast<const u32x4*>(v_base + r * v_row_bytes + (c % G::CPR) * 16);
         }
@@ -146,24 +152,29 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     auto put = [&](int buf) __attribute__((always_inline)) {
         uint8_t* dk = lds_k + buf * G::TILE_BYTES;
         uint8_t* dv = lds_v + buf * G::TILE_BYTES;
+        const bool whole = valid == ~uint64_t{0};
 #pragma unroll
         for (int i = 0; i < G::PER; ++i) {
             const int c = i * 256 + tid;
             if (G::CHUNKS % 256 != 0 && c >= G::CHUNKS) continue;
             const int r = c / G::CPR;
             const int pos = c % G::CPR;
-            const uint32_t keep = (valid >> r) & 1 ? ~0u : 0u;
+            uint32_t keep = (valid >> r) & 1 ? ~0u : 0u;
             if constexpr (kHeld8) {
                 const float ku = UnitOf(__shfl(k_byte, r)), vu = UnitOf(__shfl(v_byte, r));
                 const u32x4 k0 = Widen(kr[i].x, kr[i].y, ku), k1 = Widen(kr[i].z, kr[i].w, ku);
-                const u32x4 v0 = Widen(vr[i].x, vr[i].y, vu), v1 = Widen(vr[i].z, vr[i].w, vu);
+                u32x4 v0 = Widen(vr[i].x, vr[i].y, vu), v1 = Widen(vr[i].z, vr[i].w, vu);
+                if (!whole) {
+                    asm volatile("" : "+v"(keep));  // (a branch: as selects these are a tenth of the step's VALU work)
+                    v0 &= keep, v1 &= keep;
+                }
                 *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos) ^ SwzK<D>(r)) * 16)) = k0;
                 *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos + 1) ^ SwzK<D>(r)) * 16)) = k1;
-                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos) ^ SwzV<D>(r)) * 16)) = Masked(v0, keep);
-                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos + 1) ^ SwzV<D>(r)) * 16)) = Masked(v1, keep);
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos) ^ SwzV<D>(r)) * 16)) = v0;
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos + 1) ^ SwzV<D>(r)) * 16)) = v1;
             } else {
                 *reinterpret_cast<u32x4*>(dk + r * G::RB + ((pos ^ SwzK<D>(r)) * 16)) = kr[i];
-                *reinterpret_cast<u32x4*>(dv + r * G::RB + ((pos ^ SwzV<D>(r)) * 16)) = Masked(vr[i], keep);
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + ((pos ^ SwzV<D>(r)) * 16)) = whole ? vr[i] : vr[i] & keep;
             }
         }
     };
@@ -304,7 +315,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     }
     if (p.lse != nullptr && row_ok && hh == 0) {
         p.lse[static_cast<int64_t>(sq.q_first + token) * p.heads + head] =
-            l_all == 0.0f ? neg_inf() : (mu + __log2f(l_all)) * kLn2;
+            __builtin_bit_cast(uint32_t, l_all) == 0 ? neg_inf() : (mu + __log2f(l_all)) * kLn2;
     }
 }
 
