@@ -398,8 +398,9 @@ __device__ __forceinline__ float HalfSum(float v) {
 // 8g + 4hh + 0..3 of each group g) scaled by inv, as 16-byte chunks: the two halves of a row swap
 // words so that hh = 0 holds all of groups 0 and 2 and hh = 1 all of 1 and 3. `dst` is the row's first
 // dim of the tile (8-byte aligned); every lane of the wave takes part in the swap.
-template <typename M>
-__device__ __forceinline__ void StoreTile(uint16_t* dst, int hh, bool row_ok, const float (&v)[16]) {
+// at(c): first dim of the tile's chunk c (8 dims).
+template <typename M, typename At>
+__device__ __forceinline__ void StoreTile(uint16_t* dst, int hh, bool row_ok, const float (&v)[16], At at) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(8)));
 #pragma unroll
     for (int g = 0; g < 4; g += 2) {
@@ -408,18 +409,26 @@ __device__ __forceinline__ void StoreTile(uint16_t* dst, int hh, bool row_ok, co
         // (a, b) -> lower half: a of both halves; upper half: b of both (see HalfPair for the waits).
         asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %2\n\tv_permlane32_swap_b32 %1, %3\n\ts_nop 1"
                      : "+v"(a0), "+v"(a1), "+v"(b0), "+v"(b1));
-        if (row_ok) *reinterpret_cast<u32x4*>(dst + 8 * (g + hh)) = u32x4{a0, a1, b0, b1};
+        if (row_ok) *reinterpret_cast<u32x4*>(dst + at(g + hh)) = u32x4{a0, a1, b0, b1};
     }
+}
+template <typename M>
+__device__ __forceinline__ void StoreTile(uint16_t* dst, int hh, bool row_ok, const float (&v)[16]) {
+    StoreTile<M>(dst, hh, row_ok, v, [](int c) __attribute__((always_inline)) { return 8 * c; });
 }
 
 // The same tile unnormalised and in fp32, for a merge over key splits.
-__device__ __forceinline__ void StorePartialTile(float* dst, int hh, bool row_ok, const float (&v)[16]) {
+template <typename At>
+__device__ __forceinline__ void StorePartialTile(float* dst, int hh, bool row_ok, const float (&v)[16], At at) {
     if (!row_ok) return;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        *reinterpret_cast<float4*>(dst + 8 * g + 4 * hh) =
+        *reinterpret_cast<float4*>(dst + at(g) + 4 * hh) =
             make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
     }
+}
+__device__ __forceinline__ void StorePartialTile(float* dst, int hh, bool row_ok, const float (&v)[16]) {
+    StorePartialTile(dst, hh, row_ok, v, [](int c) __attribute__((always_inline)) { return 8 * c; });
 }
 
 // ---- Online softmax of one 32-key x 32-row S^T tile (lane: 16 keys of one row; lanes l and

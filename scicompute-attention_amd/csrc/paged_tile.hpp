@@ -9,10 +9,10 @@
 // those of the flash kernels (flash_common.hpp). Two workgroups to a CU up to D 128, so that one's
 // vector work runs beside the other's products.
 //
-// Measured (MI355X): 4 chunks of 2048 tokens behind 6,000 to 14,000, 8-bit pages, 32/8 heads, D 128: 1,735
-// us (924 TF/s; the wide kernel over 16-bit pages of the same content 1,657). Vector instructions per MFMA
-// decide: 10.3 before pool rows were multiplied in 32 bits, whole tiles left unmasked and maxima taken
-// without regard to NaN, 1,880 us. A higher wave priority over the products changes nothing.
+// Measured (MI355X): 4 chunks of 2048 tokens behind 6,000 to 14,000, 8-bit pages, 32/8 heads, D 128: 1,707
+// us (940 TF/s; the wide kernel over 16-bit pages of the same lengths 1,657). Vector instructions per MFMA
+// decide: 8.3 now, 10.3 before pool rows were multiplied in 32 bits, whole tiles left unmasked and maxima
+// taken without regard to NaN (1,880 us). A higher wave priority over the products changes nothing.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -35,6 +35,11 @@ struct TileGeom {
     static constexpr int CHUNKS = BN * CPR;
     static constexpr int PER = (CHUNKS + 255) / 256;   // chunks per thread
     static constexpr int LDS_BYTES = 4 * TILE_BYTES;   // two buffers of K and V
+    // First dim of chunk c (8 dims) of an LDS row. 8-bit pages: a lane widens 16 codes to the chunks p and
+    // p + CPR, so that the lanes of a row write neighbouring chunks (as 2p and 2p + 1 they collide in the
+    // banks: 1,724 instead of 1,707 us at the size above, D 256 570 instead of 556). Q's dims are permuted
+    // as K's are, and those of V go back to their places with the output.
+    static constexpr __device__ int ChunkDim(int c) { return !kHeld8 ? 8 * c : c < CPR ? 16 * c : 16 * (c - CPR) + 8; }
     static_assert(CHUNKS % kWave == 0, "a wave copies a chunk on all lanes or on none (shuffles)");
     static constexpr int WG_PER_CU = D <= 128 ? 2 : 1;
 };
@@ -97,10 +102,10 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
     vec8 qf[G::KS];
     {
         const uint16_t* q_row = static_cast<const uint16_t*>(p.q) +
-                                static_cast<int64_t>(sq.q_first + token) * p.q_ss + head * p.q_sh + 8 * hh;
+                                static_cast<int64_t>(sq.q_first + token) * p.q_ss + head * p.q_sh;
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks) {
-            qf[ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const uint4*>(q_row + 16 * ks));
+            qf[ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const uint4*>(q_row + G::ChunkDim(2 * ks + hh)));
         }
     }
 
@@ -168,10 +173,10 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
                     asm volatile("" : "+v"(keep));  // (a branch: as selects these are a tenth of the step's VALU work)
                     v0 &= keep, v1 &= keep;
                 }
-                *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos) ^ SwzK<D>(r)) * 16)) = k0;
-                *reinterpret_cast<u32x4*>(dk + r * G::RB + (((2 * pos + 1) ^ SwzK<D>(r)) * 16)) = k1;
-                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos) ^ SwzV<D>(r)) * 16)) = v0;
-                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((2 * pos + 1) ^ SwzV<D>(r)) * 16)) = v1;
+                *reinterpret_cast<u32x4*>(dk + r * G::RB + ((pos ^ SwzK<D>(r)) * 16)) = k0;
+                *reinterpret_cast<u32x4*>(dk + r * G::RB + (((pos + G::CPR) ^ SwzK<D>(r)) * 16)) = k1;
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + ((pos ^ SwzV<D>(r)) * 16)) = v0;
+                *reinterpret_cast<u32x4*>(dv + r * G::RB + (((pos + G::CPR) ^ SwzV<D>(r)) * 16)) = v1;
             } else {
                 *reinterpret_cast<u32x4*>(dk + r * G::RB + ((pos ^ SwzK<D>(r)) * 16)) = kr[i];
                 *reinterpret_cast<u32x4*>(dv + r * G::RB + ((pos ^ SwzV<D>(r)) * 16)) = whole ? vr[i] : vr[i] & keep;
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
             float a[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) a[i] = o[dt][i];
-            StorePartialTile(p.part_o + state * D + 32 * dt, hh, row_ok, a);
+            StorePartialTile(p.part_o + state * D, hh, row_ok, a, [&](int c) { return G::ChunkDim(4 * dt + c); });
         }
         return;
     }
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(256, (TileGeom<D, kHeld8>::WG_PER_CU)) void paged_t
         float a[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) a[i] = o[dt][i] * inv;
-        StoreTile<M>(out_row + 32 * dt, hh, row_ok, a);
+        StoreTile<M>(out_row, hh, row_ok, a, [&](int c) { return G::ChunkDim(4 * dt + c); });
     }
     if (p.lse != nullptr && row_ok && hh == 0) {
         p.lse[static_cast<int64_t>(sq.q_first + token) * p.heads + head] =
