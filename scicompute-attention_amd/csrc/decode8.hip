@@ -15,6 +15,9 @@
 //     (in fp16 a weight times a small 2^k would leave the type's range).
 //   * Exponents: one byte load per lane and tile (lanes 0-31 the tokens of K, 32-63 of V), handed to
 //     the lanes that need them with shuffles.
+//
+// Measured (MI355X): bf16, 64 sequences of 512 to 16,384 tokens, 32/8 heads, D 128: 194 us, 5.35 TB/s; 16 of
+// 3,000 to 5,200, D 96: 24.3 us (4.4); fp16, 1 x 1500, D 128: 6.5 us, a start, six tiles and a merge.
 
 #include <hip/hip_runtime.h>
 

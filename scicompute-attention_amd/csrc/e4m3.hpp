@@ -8,8 +8,8 @@
 // Why a power of two: x / 2^k and code * 2^k are exact, so that a code does not depend on how a
 // division rounds, and every product code * 2^k is itself a number of the 16-bit type: attention
 // over 8-bit pages is attention over 16-bit values, converted in registers with no rounding of its
-// own. An e4m3 value has as many bits whatever its size, so that only values below 2^-14 of the
-// row's largest notice the coarser scale.
+// own. An e4m3 value has as many bits whatever its size, so that only values below about 2^-14 of
+// the row's largest notice the coarser scale.
 //
 // Magnitudes above 1.875 times the type's largest power of two (61440 in fp16) would round to the
 // next power of two, which the type does not have: they are held as that value (off by less than
@@ -30,7 +30,6 @@ struct Held;  // conversions of one 16-bit type
 
 template <>
 struct Held<F16> {
-    typedef _Float16 pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kLargest = 61440.0f;
     // Codes 2 * half and 2 * half + 1 of the word times `unit` (a power of two), as a packed pair.
     template <bool kHalf>
@@ -41,7 +40,6 @@ struct Held<F16> {
 
 template <>
 struct Held<BF16> {
-    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
     static constexpr float kLargest = 0x1.ep127f;
     template <bool kHalf>
     static __device__ __forceinline__ uint32_t widen2(uint32_t codes, float unit) {

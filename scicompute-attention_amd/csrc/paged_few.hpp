@@ -10,6 +10,10 @@
 //   O^T[D x 16 NC rows] += V^T P^T, V through this wave's own LDS tile and transposed reads.
 // 8-bit codes are widened (e4m3.hpp) between memory and the matrix unit. A wave has one tile in flight:
 // the next V is requested when V has gone to LDS, the next K behind the QK products.
+//
+// Measured (MI355X): bf16, 8 sequences of 6 tokens behind 4,096, 32/8 heads, D 128: 30 us, 4.5 TB/s (a
+// call 43; through the 128-row kernel of paged_tile.hpp, 24 of its rows in use, 93); fp16, 40 single
+// tokens behind 200 to 6,000, D 64: 49 us, 5.2 TB/s; 5 tokens behind 2,300, 8-bit pages: 9.3 us.
 #pragma once
 
 #include <hip/hip_runtime.h>

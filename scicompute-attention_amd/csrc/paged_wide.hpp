@@ -1,7 +1,12 @@
 // Long chunks of new tokens over 16-bit pages (paged_varlen.hpp): the wide-row flash kernel
 // (flash_wide.hpp, head_dim 32 to 160) with its K and V tiles copied page by page. A wave copies 16
 // rows of every 64-key tile, so pages of at least 16 tokens serve it: their ids are uniform per wave,
-// come through the scalar cache and cost no vector instruction.
+// come through the scalar cache and cost no vector instruction. The matrix units and the softmax's vector
+// work bound it, as they bound the kernel over plain K and V.
+//
+// Measured (MI355X): bf16, 512 tokens behind 12,289, 32/8 heads, D 128: 126 us with the merge (paged_tile.hpp
+// over the same pages 320; K and V without pages 107); 4 chunks of 2048 behind 6,000 to 14,000: 1,657
+// us, 968 TF/s; 3 of 300 to 1000 behind 200 to 6,000, D 64: 75 us.
 #pragma once
 
 #include <hip/hip_runtime.h>
