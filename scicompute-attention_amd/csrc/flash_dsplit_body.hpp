@@ -133,8 +133,9 @@
     const int page_key0 = static_cast<int>(key0);
     const PagedKeys pages(job);
     if constexpr (kPaged) {
-        // Tiles from the first page on that is not mapped are masked.
-        n_plain = min(n_plain, (FirstHole(pages, job.table, page_key0, page_key0 + rows) - page_key0) / BN);
+        // Tiles from the first page on that is not mapped are masked. (n_plain is negative where the first rows
+        // come before the first key: more new tokens than keys.)
+        n_plain = max(0, min(n_plain, (FirstHole(pages, job.table, page_key0, page_key0 + rows) - page_key0) / BN));
     }
     auto rows_of = [&](int t, int id) __attribute__((always_inline)) -> PagedRows {
         return RowsAt(pages, page_key0 + t * BN + wave * kPagedRowsPerWave, id, kPagedRowsPerWave, page_key0 + rows);

@@ -143,9 +143,10 @@
     const int key0 = static_cast<int>(tok_kv);  // of tile 0
     const PagedKeys pages(job);
     if constexpr (kMode == kPaged) {
-        // Tiles from the first page on that is not mapped are masked.
+        // Tiles from the first page on that is not mapped are masked. (n_plain is negative where the first rows
+        // come before the first key: more new tokens than keys.)
         const int end = key0 + min(seq_kv, n_tiles * BN);
-        n_plain = min(n_plain, (FirstHole(pages, job.table, key0, end) - key0) / BN);
+        n_plain = max(0, min(n_plain, (FirstHole(pages, job.table, key0, end) - key0) / BN));
     }
     auto rows_of = [&](int t, int id) __attribute__((always_inline)) -> PagedRows {
         return RowsAt(pages, key0 + t * BN + wave * kPagedRowsPerWave, id, kPagedRowsPerWave, 0x7fffffff);

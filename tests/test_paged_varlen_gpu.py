@@ -186,6 +186,14 @@ def test_rows_that_see_no_key(hip, D, held8):
 
 
 @pytest.mark.parametrize("held8", STORED)
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 256])
+def test_tiles_of_rows_before_the_first_key(hip, D, held8):
+    """More new tokens than keys by more than a tile of them."""
+    case([16, 200, 0], [58, 430, 90], 16, 20, 1, D, "f16", held8, 2750 + D)
+    case([3, 40], [300, 129], 16, 2, 2, D, "bf16", held8, 2760 + D)
+
+
+@pytest.mark.parametrize("held8", STORED)
 @pytest.mark.parametrize("D", [64, 128, 192])
 def test_nan_keys_reach_their_rows_and_no_others(hip, D, held8):
     pl = pool([600, 600], 16, 2, D, "bf16", 2800, held8)
