@@ -180,7 +180,7 @@ template <typename E, int D, bool kCausal>
 int LaunchFlashVarlen(const sca_flash_varlen_params& v, hipStream_t s);  // flash_wide.hpp
 
 // A workgroup's share of a launch over paged KV: packed rows of one row tile and KV head, and
-// a range of key tiles. Pages of at least 16 tokens.
+// a range of key tiles. Pages of at least 16 tokens (8 in the split-dims kernel).
 struct PagedJob {
     const int32_t* table;   // the sequence's row of the page table
     int64_t max_blocks, num_blocks;

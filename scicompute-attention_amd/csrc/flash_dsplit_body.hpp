@@ -143,16 +143,25 @@
     auto own_id = [&](int t) __attribute__((always_inline)) -> int {
         return pages.id(page_key0 + t * BN + wave * kPagedRowsPerWave);
     };
-    // Holes of tile t (keys on pages that are not mapped): bit g for keys 16 g .. + 16.
-    auto half_id = [&](int t, int g) __attribute__((always_inline)) -> int {
-        return pages.id(page_key0 + t * BN + 16 * g);
+    // Holes of tile t (keys on pages that are not mapped): bit g for keys 8 g .. + 8.
+    struct Ids {
+        int of[4];
     };
-    auto holes_of = [&](int t, int id0, int id1) __attribute__((always_inline)) -> int {
-        const int key = page_key0 + t * BN;
-        return (pages.hole(key, id0) ? 1 : 0) | (pages.hole(key + 16, id1) ? 2 : 0);
+    auto ids_of = [&](int t) __attribute__((always_inline)) -> Ids {
+        Ids ids;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) ids.of[g] = pages.id(page_key0 + t * BN + 8 * g);
+        return ids;
+    };
+    auto holes_of = [&](int t, const Ids& ids) __attribute__((always_inline)) -> int {
+        int holes = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) holes |= pages.hole(page_key0 + t * BN + 8 * g, ids.of[g]) ? 1 << g : 0;
+        return holes;
     };
     PagedRows rows_v{0, 0}, rows_mid{0, 0}, rows_k{0, 0};  // of tiles t + 4, t + 5 and t + 6 in step t
-    int id_own = 0, id_half0 = 0, id_half1 = 0;
+    int id_own = 0;
+    Ids tile_ids{};
     // DMA instruction i of this wave's share of K tile t (into K slot t & 3) or V tile t.
     auto dma_k = [&](int i, int slot, int t) __attribute__((always_inline)) {
         if constexpr (kPaged) {
@@ -245,7 +254,7 @@
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = kbase + 8 * (i / 4) + (i % 4);
-                sr[i] = key > lim || (kPaged && ((holes >> (i / 8)) & 1)) ? neg_inf() : sr[i];
+                sr[i] = key > lim || (kPaged && ((holes >> (i / 4)) & 1)) ? neg_inf() : sr[i];
             }
         }
         return Max16(sr);
@@ -324,12 +333,12 @@
         int ids[6];
 #pragma unroll
         for (int i = 0; i < 6; ++i) ids[i] = own_id(i);
-        const int a0 = half_id(0, 0), a1 = half_id(0, 1), b0 = half_id(1, 0), b1 = half_id(1, 1);
+        const Ids ids0 = ids_of(0), ids1 = ids_of(1);
         id_own = own_id(6);
 #pragma unroll
         for (int i = 0; i < 6; ++i) first_rows[i] = rows_of(i, ids[i]);
-        holes0 = holes_of(0, a0, a1);
-        holes1 = holes_of(1, b0, b1);
+        holes0 = holes_of(0, ids0);
+        holes1 = holes_of(1, ids1);
     }
     auto issue = [&](int t_k, int t_v) __attribute__((always_inline)) {
         if constexpr (kPaged) {
@@ -426,9 +435,8 @@
             rows_k = rows_of(t + 6, id_own);
             id_own = own_id(t + 7);
             if constexpr (kMaskable) {
-                next_holes = holes_of(t + 2, id_half0, id_half1);
-                id_half0 = half_id(t + 3, 0);
-                id_half1 = half_id(t + 3, 1);
+                next_holes = holes_of(t + 2, tile_ids);
+                tile_ids = ids_of(t + 3);
             }
         }
         // ---- A ----
@@ -516,10 +524,7 @@
         step.template operator()<false, 2>(t + 2, s1, s0, pb0, pb1);
         step.template operator()<false, 3>(t + 3, s0, s1, pb1, pb0);
     }
-    if constexpr (kPaged) {
-        id_half0 = half_id(t + 2, 0);
-        id_half1 = half_id(t + 2, 1);
-    }
+    if constexpr (kPaged) tile_ids = ids_of(t + 2);
     for (; t < n_tiles; t += 4) {
         step.template operator()<true, 0>(t, s1, s0, pb0, pb1);
         if (t + 1 >= n_tiles) break;

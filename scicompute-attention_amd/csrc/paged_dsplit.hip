@@ -1,6 +1,6 @@
 // Long chunks of new tokens over 16-bit pages at head_dim 192 and 256: the split-dims flash kernel
 // (flash_dsplit.hip) with its K and V tiles copied page by page, as paged_wide.hpp does for the smaller
-// head dims. A wave copies 8 rows of every 32-key tile.
+// head dims. A wave copies 8 rows of every 32-key tile, so pages of 8 tokens will do.
 //
 // Measured (MI355X): three prompts of 900 to 2600 tokens, 16/4 heads, D 256, LSE: 225 us (paged_tile.hpp)
 // -> 115 us. Looking at the page ids of every tile inside the steady loop, instead of once ahead of it

@@ -1,13 +1,13 @@
 // The general kernel of attention over paged KV (paged_varlen.hpp): 8-bit pages, pages of fewer than 16
-// tokens, and rows of pages more than 2^25 elements apart. The matrix units bound it.
+// tokens (8 from head_dim 192 on), and rows of pages more than 2^25 elements apart. The matrix units bound it.
 //
-// Four waves of 32 packed rows; key tiles of 64 keys (32 from head_dim 160 on) come through registers
+// Four waves of 32 packed rows; key tiles of 64 or 32 keys (TileKeys) come through registers
 // into two LDS buffers: while a tile is multiplied the next one's loads are in flight, and 8-bit codes
 // are widened (e4m3.hpp) on their way into LDS, once per workgroup, so that one inner loop serves both
 // kinds of pages. A lane looks up the page of one key per tile, one tile ahead of the loads that need it,
 // and hands the row to the lanes that copy it with a shuffle. Formulation, swizzles and online softmax are
-// those of the flash kernels (flash_common.hpp). Two workgroups to a CU up to D 128, so that one's
-// vector work runs beside the other's products.
+// those of the flash kernels (flash_common.hpp). Two workgroups to a CU where they fit (TileResident), so that
+// one's vector work runs beside the other's products.
 //
 // Measured (MI355X): 4 chunks of 2048 tokens behind 6,000 to 14,000, 8-bit pages, 32/8 heads, D 128: 1,707
 // us (940 TF/s; the wide kernel over 16-bit pages of the same lengths 1,657). Vector instructions per MFMA
@@ -25,7 +25,7 @@ namespace {
 
 template <int D, bool kHeld8>
 struct TileGeom {
-    static constexpr int BN = D <= 128 ? 64 : 32;      // keys per tile
+    static constexpr int BN = TileKeys(D, kHeld8);     // keys per tile
     static constexpr int NT = BN / 32;                 // S^T tiles of 32 keys
     static constexpr int KS = D / 16;
     static constexpr int DT = D / 32;
@@ -41,7 +41,7 @@ struct TileGeom {
     // as K's are, and those of V go back to their places with the output.
     static constexpr __device__ int ChunkDim(int c) { return !kHeld8 ? 8 * c : c < CPR ? 16 * c : 16 * (c - CPR) + 8; }
     static_assert(CHUNKS % kWave == 0, "a wave copies a chunk on all lanes or on none (shuffles)");
-    static constexpr int WG_PER_CU = D <= 128 ? 2 : 1;
+    static constexpr int WG_PER_CU = TileResident(D, kHeld8);
 };
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (a plain vector stays in registers)

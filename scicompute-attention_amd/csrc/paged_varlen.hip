@@ -116,8 +116,9 @@ struct Plan {
 Kind KindFor(const sca_paged_varlen_params& p, int64_t rows) {
     if (rows <= 16) return kFew16;
     if (rows <= 32) return p.head_dim <= 192 ? kFew32 : kFew16;
-    // (the flash kernels address 16 rows of a page with 32-bit offsets)
-    const bool flash = p.k_exp == nullptr && p.block_size >= 16 && p.k_ss < (1 << 25) && p.v_ss < (1 << 25);
+    // (the flash kernels copy 16 or 8 rows of a page at a time, and address them with 32-bit offsets)
+    const bool flash = p.k_exp == nullptr && p.block_size >= (p.head_dim <= 160 ? 16 : 8) && p.k_ss < (1 << 25) &&
+                       p.v_ss < (1 << 25);
     return flash ? kFlash : kTile;
 }
 
@@ -125,15 +126,16 @@ bool IsFew(Kind kind) { return kind == kFew16 || kind == kFew32; }
 int RowsPerTile(Kind kind) { return !IsFew(kind) ? kPagedRows : kind == kFew32 ? 32 : 16; }
 
 // Keys that a workgroup takes in one step.
-int KeysPerStep(Kind kind, int64_t head_dim) {
-    return IsFew(kind) ? 128 : head_dim <= (kind == kFlash ? 160 : 128) ? 64 : 32;
+int KeysPerStep(Kind kind, const sca_paged_varlen_params& p) {
+    const int d = static_cast<int>(p.head_dim);
+    return IsFew(kind) ? 128 : kind == kTile ? TileKeys(d, p.k_exp != nullptr) : d <= 160 ? 64 : 32;
 }
 
 // Workgroups that the GPU holds at once.
 int64_t Resident(Kind kind, const sca_paged_varlen_params& p) {
     const int d = static_cast<int>(p.head_dim);
     const int on_cu = kind == kFlash   ? (d <= 64 ? 2 : 1)
-                      : kind == kTile ? (d <= 128 ? 2 : 1)
+                      : kind == kTile ? TileResident(d, p.k_exp != nullptr)
                                       : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
     return static_cast<int64_t>(CuCount()) * on_cu;
 }
@@ -203,7 +205,7 @@ int64_t Makespan(const std::vector<Entry>& list, const sca_paged_varlen_params& 
 void PlanKind(const sca_paged_varlen_params& p, Kind kind, int64_t most_states, Plan* plan) {
     const int64_t group = p.num_heads / p.num_kv_heads;
     const int64_t rows_per_tile = RowsPerTile(kind);
-    const int64_t keys = KeysPerStep(kind, p.head_dim);
+    const int64_t keys = KeysPerStep(kind, p);
     std::vector<Entry> list;
     int64_t work = 0;  // steps of all units
     for (int64_t s = 0; s < p.num_seqs; ++s) {

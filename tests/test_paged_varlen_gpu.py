@@ -254,6 +254,16 @@ def test_unmapped_pages_under_long_chunks(hip, D):
         case([L], [90], 16, 1, 1, D, "bf16", False, 3320 + n, mutate=mutate, scratches=(True,), causal=False)
 
 
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_unmapped_pages_of_eight_tokens_under_long_chunks(hip, D):
+    for n, (L, holes) in enumerate([(300, (0,)), (1000, (1, 3, 33, 62, 100)), (1000, (124,)), (6000, (700, 749))]):
+        def mutate(pl):
+            for i, h in enumerate(holes):
+                pl["table"][0, h] = -1 if i % 2 == 0 else pl["nb"]
+        case([L], [70], 8, 2, 2, D, "f16" if n % 2 else "bf16", False, 3360 + n, mutate=mutate)
+        case([L], [70], 8, 1, 1, D, "bf16", False, 3370 + n, mutate=mutate, scratches=(True,), causal=False)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("D", [32, 64, 96])
 def test_chunks_and_single_tokens_in_one_step(hip, D, dtype):
