@@ -137,7 +137,7 @@ int KeysPerStep(Kind kind, const sca_paged_varlen_params& p) {
 int64_t Resident(Kind kind, const sca_paged_varlen_params& p) {
     const int d = static_cast<int>(p.head_dim);
     const int on_cu = kind == kFlash   ? (d <= 64 ? 2 : 1)
-                      : kind == kTile ? TileResident(d, p.k_exp != nullptr)
+                      : kind == kTile ? TileResident(d)
                                       : FewResident(d, p.k_exp != nullptr, kind == kFew32 ? 2 : 1);
     return static_cast<int64_t>(CuCount()) * on_cu;
 }

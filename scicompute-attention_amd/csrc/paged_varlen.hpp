@@ -31,13 +31,14 @@ constexpr int FewResident(int head_dim, bool held8, int column_groups) {
     return need <= 96 ? 5 : need <= 128 ? 4 : need <= 168 ? 3 : need <= 256 ? 2 : 1;
 }
 
-// Keys per tile of the general kernel and workgroups of it that a CU holds, by what fits 256 registers a lane
-// (all 512 with one workgroup). Measured (2 chunks of 1024 tokens behind 6,000 to 9,000, MI355X, us), 64 or 32
-// keys: 16-bit D 96 145 / 167, D 128 502 / 331, 8-bit D 128 (4 of 2048) 1,707 / 1,809; one or two workgroups:
-// D 160 16-bit 421 / 238, 8-bit (5 of 856 behind 8,535) 1,360 / 810, D 192 16-bit 813 / 1,129, 8-bit (3 of
-// 1,295 to 3,885) 622 / 588, D 256 8-bit 556 / 1,153.
-constexpr int TileKeys(int head_dim, bool held8) { return head_dim <= (held8 ? 128 : 96) ? 64 : 32; }
-constexpr int TileResident(int head_dim, bool held8) { return head_dim <= (held8 ? 192 : 160) ? 2 : 1; }
+// Keys per tile of the general kernel and workgroups of it that a CU holds, by what fits 256 registers a lane.
+// Measured (MI355X, us), 64 or 32 keys: 16-bit D 96 145 / 167, D 128 502 / 331 (2 chunks of 1024 tokens behind
+// 6,000 to 9,000), 8-bit D 128 (4 of 2048) 1,707 / 1,809; one or two workgroups: D 160 16-bit 421 / 238, 8-bit (5
+// of 856 behind 8,535) 1,360 / 810. From D 192 on a workgroup has eight waves.
+constexpr int TileKeys(int head_dim, bool held8) {
+    return head_dim <= (held8 ? 128 : 96) || head_dim >= 192 ? 64 : 32;
+}
+constexpr int TileResident(int head_dim) { return head_dim <= 160 ? 2 : 1; }
 
 struct PagedSeq {
     int32_t unit_end;    // units of this and all earlier sequences of the launch
